@@ -50,7 +50,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
         return LIB
     tmp = LIB + ".tmp"
     cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-           "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr",
+           "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr", "--threads", "0",
            "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-o", tmp, *sources()]
     if ptxas_verbose:
         cmd[1:1] = ["-Xptxas", "-v"]

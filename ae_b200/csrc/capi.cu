@@ -9,6 +9,7 @@
 #include <mutex>
 
 #include "../../include/ae_b200.h"
+#include "host.h"
 #include "kernels.h"
 
 using namespace smb;
@@ -17,15 +18,19 @@ namespace {
 
 thread_local char g_last_cuda_error[256] = "";
 
+}  // namespace
+
+namespace smb {
+
 int cuda_fail(cudaError_t err) {
   std::snprintf(g_last_cuda_error, sizeof(g_last_cuda_error), "%s: %s", cudaGetErrorName(err),
                 cudaGetErrorString(err));
   return SMB_ERR_CUDA;
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+}  // namespace smb
+
+namespace {
 
 typedef CUresult (*StreamWriteValue32Fn)(CUstream, CUdeviceptr, cuuint32_t, unsigned int);
 
@@ -45,6 +50,10 @@ StreamWriteValue32Fn write_value_fn() {
   return fn;
 }
 
+}  // namespace
+
+namespace smb {
+
 EncodeTiledFn encode_fn() {
   static EncodeTiledFn fn = nullptr;
   static std::once_flag once;
@@ -58,11 +67,6 @@ EncodeTiledFn encode_fn() {
   });
   return fn;
 }
-
-struct DeviceInfo {
-  int sms = 0;
-  bool sm100 = false;
-};
 
 constexpr int kMaxDevices = 64;
 
@@ -99,6 +103,10 @@ bool pdl_enabled() {
   }();
   return on;
 }
+
+}  // namespace smb
+
+namespace {
 
 int elem_bytes_of(int dtype) { return (dtype == SMB_DTYPE_F16 || dtype == SMB_DTYPE_BF16) ? 2 : 0; }
 
@@ -545,16 +553,18 @@ int smb_version(void) { return 100; }
 const char* smb_strerror(int code) {
   switch (code) {
     case SMB_OK: return "ok";
-    case SMB_ERR_SHAPE: return "unsupported size (need H%128==0, I%64==0, 1<=E<=256, 1<=k<=min(E,8), T*k<=16384)";
+    case SMB_ERR_SHAPE:
+      return "unsupported size (MoE: H%128==0, I%64==0, 1<=E<=256, 1<=k<=min(E,8), T*k<=16384; paged cache: head size "
+             "64, 128 or 256, page size a power of two, query heads a multiple of key heads)";
     case SMB_ERR_DTYPE: return "unsupported dtype (storage f16/bf16; logits f16/bf16/f32)";
     case SMB_ERR_ALIGN: return "misaligned pointer (tensors 16 B, workspace 256 B)";
-    case SMB_ERR_WORKSPACE: return "workspace smaller than smb_moe_workspace_bytes";
+    case SMB_ERR_WORKSPACE: return "workspace smaller than its size function asks for";
     case SMB_ERR_CUDA: return "CUDA runtime error (see smb_last_cuda_error)";
     case SMB_ERR_TMA: return "tensor-map encoding failed";
     case SMB_ERR_ARCH: return "current device is not sm_100 (B200)";
     case SMB_ERR_NULL: return "required pointer is NULL";
     case SMB_ERR_DEVICE_TIMEOUT: return "device pipeline wait exceeded its budget";
-    case SMB_ERR_BAD_PAGE: return "page_of_expert entry outside [0, num_pages)";
+    case SMB_ERR_BAD_PAGE: return "page outside [0, num_pages)";
     case SMB_ERR_BAD_EXPERT: return "expert id outside [0, E)";
     case SMB_ERR_SCRATCH_LIMIT: return "workspace need exceeds the 64 MiB static scratch of smb_moe_forward_noalloc";
     default: return "unknown error";

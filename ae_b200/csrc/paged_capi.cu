@@ -1,0 +1,212 @@
+// C ABI entry points of the paged key/value cache: argument checks and launches.
+#include "../../include/ae_b200.h"
+#include "host.h"
+#include "paged.h"
+
+using namespace smb;
+
+namespace {
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool storage(int dtype) { return dtype == SMB_DTYPE_F16 || dtype == SMB_DTYPE_BF16; }
+
+int cache_args(const smb_paged_cache_t* c, PagedCacheArgs* out) {
+  if (c == nullptr) return SMB_ERR_NULL;
+  if (c->bits != 16 && c->bits != 4) return SMB_ERR_DTYPE;
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return SMB_ERR_SHAPE;
+  if (c->kv_heads < 1 || c->kv_heads > kPagedMaxHeads || c->num_pages < 0) return SMB_ERR_SHAPE;
+  if (c->page_size < 1 || c->page_size > kPagedMaxPage || (c->page_size & (c->page_size - 1)) != 0) return SMB_ERR_SHAPE;
+  if (c->page_stride < 0 || c->head_stride < 0 || c->token_stride < 0) return SMB_ERR_SHAPE;
+  if (c->page_stride % 16 || c->head_stride % 16 || c->token_stride % 16) return SMB_ERR_ALIGN;
+  if (!aligned16(c->k) || !aligned16(c->v)) return SMB_ERR_ALIGN;
+  if (c->num_pages > 0 && (c->k == nullptr || c->v == nullptr)) return SMB_ERR_NULL;
+  out->k = static_cast<uint8_t*>(c->k);
+  out->v = static_cast<uint8_t*>(c->v);
+  out->num_pages = c->num_pages;
+  out->page_stride = c->page_stride;
+  out->head_stride = c->head_stride;
+  out->token_stride = c->token_stride;
+  out->page_shift = __builtin_ctz(static_cast<unsigned>(c->page_size));
+  out->Hkv = c->kv_heads;
+  return SMB_OK;
+}
+
+int need_b200(DeviceInfo* di) {
+  const int rc = device_info(di);
+  if (rc != SMB_OK) return rc;
+  return di->sm100 ? SMB_OK : SMB_ERR_ARCH;
+}
+
+int done(cudaError_t err) { return err == cudaSuccess ? SMB_OK : cuda_fail(err); }
+
+// Sizes of an attention call, checked.
+int attn_sizes(int N, int B, int Hq, int Hkv, int D, int bits) {
+  if (D != 64 && D != 128 && D != 256) return SMB_ERR_SHAPE;
+  if (bits != 16 && bits != 4) return SMB_ERR_DTYPE;
+  if (N < 0 || B < 0 || Hkv < 1 || Hq < Hkv || Hq % Hkv != 0 || Hq > kPagedMaxHeads) return SMB_ERR_SHAPE;
+  if (static_cast<long long>(N) * Hq > 0x7fffffffll) return SMB_ERR_SHAPE;
+  return SMB_OK;
+}
+
+size_t attn_ws(const AttnPlan& p, int D) {
+  return static_cast<size_t>(2) * p.grid * p.rows * (D + 2) * sizeof(float);
+}
+
+}  // namespace
+
+extern "C" {
+
+int smb_kv4_row_bytes(int head_dim) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return SMB_ERR_SHAPE;
+  return kv4_row_bytes(head_dim);
+}
+
+int smb_kv_append(const smb_paged_cache_t* cache, const void* q, const void* k, const void* v, const int64_t* strides,
+                  int dtype, int N, int Hq, const int64_t* slots, const int64_t* positions, const double* inv_freq,
+                  int rot, int interleaved, float rope_scale, const void* q_norm, const void* k_norm, float eps,
+                  void* q_out, int* status, smb_stream_t stream) {
+  AppendArgs a{};
+  int rc = cache_args(cache, &a.c);
+  if (rc != SMB_OK) return rc;
+  if (!storage(dtype)) return SMB_ERR_DTYPE;
+  const int D = cache->head_dim;
+  if (N < 0 || Hq < 1 || Hq > kPagedMaxHeads || rot < 0 || rot > D || rot % 16 != 0) return SMB_ERR_SHAPE;
+  if (N == 0) return SMB_OK;
+  if (q == nullptr || k == nullptr || v == nullptr || strides == nullptr || slots == nullptr || q_out == nullptr)
+    return SMB_ERR_NULL;
+  if (rot > 0 && (positions == nullptr || inv_freq == nullptr)) return SMB_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(q_norm) || !aligned16(k_norm))
+    return SMB_ERR_ALIGN;
+  for (int i = 0; i < 6; ++i)
+    if (strides[i] % 8 != 0) return SMB_ERR_ALIGN;
+  DeviceInfo di;
+  rc = need_b200(&di);
+  if (rc != SMB_OK) return rc;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_ts = strides[0];
+  a.q_hs = strides[1];
+  a.k_ts = strides[2];
+  a.k_hs = strides[3];
+  a.v_ts = strides[4];
+  a.v_hs = strides[5];
+  a.slots = reinterpret_cast<const long long*>(slots);
+  a.positions = reinterpret_cast<const long long*>(positions);
+  a.inv_freq = inv_freq;
+  a.rot = rot;
+  a.interleaved = interleaved;
+  a.rope_scale = rope_scale;
+  a.eps = eps;
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.q_out = q_out;
+  a.status = status;
+  a.N = N;
+  a.Hq = Hq;
+  return done(launch_kv_append(a, D, dtype == SMB_DTYPE_BF16, cache->bits == 4, di.sms,
+                               reinterpret_cast<cudaStream_t>(stream), pdl_enabled()));
+}
+
+int smb_kv4_read(const void* cache, int64_t num_pages, int kv_heads, int page_size, int head_dim, int64_t page_stride,
+                 int64_t head_stride, int64_t token_stride, int dtype, const int64_t* slots, int M, void* out,
+                 smb_stream_t stream) {
+  smb_paged_cache_t c{};
+  c.k = c.v = const_cast<void*>(cache);
+  c.num_pages = num_pages;
+  c.page_stride = page_stride;
+  c.head_stride = head_stride;
+  c.token_stride = token_stride;
+  c.kv_heads = kv_heads;
+  c.page_size = page_size;
+  c.head_dim = head_dim;
+  c.bits = 4;
+  PagedCacheArgs ca;
+  int rc = cache_args(&c, &ca);
+  if (rc != SMB_OK) return rc;
+  if (!storage(dtype)) return SMB_ERR_DTYPE;
+  if (M < 0) return SMB_ERR_SHAPE;
+  if (M == 0) return SMB_OK;
+  if (slots == nullptr || out == nullptr) return SMB_ERR_NULL;
+  if (!aligned16(out)) return SMB_ERR_ALIGN;
+  DeviceInfo di;
+  rc = need_b200(&di);
+  if (rc != SMB_OK) return rc;
+  Kv4ReadArgs a{};
+  a.cache = ca.k;
+  a.num_pages = ca.num_pages;
+  a.page_stride = ca.page_stride;
+  a.head_stride = ca.head_stride;
+  a.token_stride = ca.token_stride;
+  a.page_shift = ca.page_shift;
+  a.Hkv = ca.Hkv;
+  a.slots = reinterpret_cast<const long long*>(slots);
+  a.M = M;
+  a.out = out;
+  return done(launch_kv4_read(a, head_dim, dtype == SMB_DTYPE_BF16, reinterpret_cast<cudaStream_t>(stream), pdl_enabled()));
+}
+
+size_t smb_paged_attention_workspace_bytes(int N, int B, int Hq, int Hkv, int head_dim, int bits) {
+  if (attn_sizes(N, B, Hq, Hkv, head_dim, bits) != SMB_OK) return 0;
+  DeviceInfo di;
+  if (device_info(&di) != SMB_OK) return 0;
+  if (N == 0 || B == 0) return 256;
+  return attn_ws(plan_attn_mma(N, B, Hq / Hkv, head_dim, bits == 4, di.sms), head_dim);
+}
+
+int smb_paged_attention(const smb_paged_cache_t* cache, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                        int dtype, int N, int Hq, int B, const int32_t* block_table, int64_t table_stride,
+                        int max_pages, const int32_t* kv_lens, const int32_t* q_starts, const int32_t* tree,
+                        int64_t tree_stride, int tree_words, float scale, void* out, int64_t out_token_stride,
+                        int64_t out_head_stride, float* lse, int* status, void* ws, size_t ws_bytes,
+                        smb_stream_t stream) {
+  AttnArgs a{};
+  int rc = cache_args(cache, &a.c);
+  if (rc != SMB_OK) return rc;
+  if (!storage(dtype)) return SMB_ERR_DTYPE;
+  const int D = cache->head_dim;
+  rc = attn_sizes(N, B, Hq, a.c.Hkv, D, cache->bits);
+  if (rc != SMB_OK) return rc;
+  if (max_pages < 0 || table_stride < 0 || (tree != nullptr && (tree_words < 1 || tree_stride < 0))) return SMB_ERR_SHAPE;
+  if (N == 0 || B == 0) return SMB_OK;
+  if (q == nullptr || out == nullptr || kv_lens == nullptr || q_starts == nullptr || ws == nullptr) return SMB_ERR_NULL;
+  if (max_pages > 0 && block_table == nullptr) return SMB_ERR_NULL;
+  if (!aligned16(q) || !aligned16(out) || !aligned16(ws)) return SMB_ERR_ALIGN;
+  if (q_token_stride % 8 || q_head_stride % 8 || out_token_stride % 8 || out_head_stride % 8) return SMB_ERR_ALIGN;
+  DeviceInfo di;
+  rc = need_b200(&di);
+  if (rc != SMB_OK) return rc;
+  a.q = q;
+  a.q_ts = q_token_stride;
+  a.q_hs = q_head_stride;
+  a.N = N;
+  a.B = B;
+  a.g = Hq / a.c.Hkv;
+  a.table = block_table;
+  a.table_stride = table_stride;
+  a.max_pages = max_pages;
+  a.kv_lens = kv_lens;
+  a.q_starts = q_starts;
+  a.tree = tree;
+  a.tree_stride = tree_stride;
+  a.tree_words = tree_words;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = out;
+  a.o_ts = out_token_stride;
+  a.o_hs = out_head_stride;
+  a.lse = lse;
+  a.status = status;
+  const bool bits4 = cache->bits == 4;
+  const AttnPlan p = plan_attn_mma(N, B, a.g, D, bits4, di.sms);
+  if (ws_bytes < attn_ws(p, D)) return SMB_ERR_WORKSPACE;
+  a.gs = a.g < p.rows ? a.g : p.rows;
+  a.nsub = (a.g + a.gs - 1) / a.gs;
+  a.tq = p.rows / a.gs;
+  a.part_o = static_cast<float*>(ws);
+  a.part_ml = a.part_o + static_cast<size_t>(2) * p.grid * p.rows * D;
+  a.min_tiles = 2;
+  return done(launch_attn_mma(a, p, D, dtype == SMB_DTYPE_BF16, bits4, reinterpret_cast<cudaStream_t>(stream),
+                              pdl_enabled()));
+}
+
+}  // extern "C"

@@ -1,0 +1,206 @@
+// How one attention call's work is cut over a grid, computed by every CTA from the lengths on
+// the device (the host does not know them).
+//
+// A segment is (sequence b, key head or part of one vh, row tile qt): the rows of tq tokens x gs
+// query heads against the keys those tokens can see, in tiles of BK keys.  The tiles of all
+// segments in the order (b, vh, qt, tile) form one line of W tiles, and CTA c takes the tiles
+// [W c / G, W (c + 1) / G): whatever the lengths, the CTAs' shares differ by one tile.  A segment
+// that lies inside one share is finished by its CTA; one that is cut leaves a partial result in
+// at most two slots per CTA (2c: the segment its share begins in, 2c + 1: the one it ends in),
+// and a second kernel joins the parts in the order of their CTAs, so the result does not depend
+// on timing.  The slots' size follows the grid and not the lengths.
+#pragma once
+
+#include "common.cuh"
+#include "paged.h"
+
+namespace smb {
+
+constexpr int kPlanThreads = 128;  // threads that share the scan over the sequences
+
+struct Seq {
+  int s0, n, L;  // first row of q, new tokens, keys
+};
+
+__device__ __forceinline__ Seq seq_at(const AttnArgs& a, int b) {
+  Seq s;
+  const int lo = min(max(a.q_starts[b], 0), a.N);
+  const int hi = min(max(a.q_starts[b + 1], lo), a.N);
+  s.s0 = lo;
+  s.n = hi - lo;
+  const long long cap = min(static_cast<long long>(a.max_pages) << a.c.page_shift, 0x7fffffffll);
+  s.L = min(max(a.kv_lens[b], 0), static_cast<int>(cap));
+  return s;
+}
+
+__device__ __forceinline__ int row_tiles(const AttnArgs& a, const Seq& s) { return (s.n + a.tq - 1) / a.tq; }
+
+// Keys that row tile qt can see (all of them for a tree, up to its last token otherwise).
+__device__ __forceinline__ int keys_of_tile(const AttnArgs& a, const Seq& s, int qt) {
+  if (a.tree != nullptr) return s.L;
+  const long long end = static_cast<long long>(s.L) - s.n + min(static_cast<long long>(s.n), (qt + 1ll) * a.tq);
+  return static_cast<int>(max(end, 0ll));
+}
+
+template <int BK>
+__device__ __forceinline__ int tiles_of(int keys) {
+  return max(1, keys / BK + (keys % BK != 0));
+}
+
+// sum over i < n of floor((step * i + b) / BK), b >= 0
+template <int BK>
+__device__ __forceinline__ long long floor_sum(long long n, long long step, long long b) {
+  long long sum = 0, m = BK, a = step;
+  while (n > 0) {
+    sum += (n - 1) * n / 2 * (a / m) + n * (b / m);
+    a %= m;
+    b %= m;
+    const long long y = a * n + b;
+    if (y < m) break;
+    n = y / m;
+    b = y % m;
+    const long long t = m;
+    m = a;
+    a = t;
+  }
+  return sum;
+}
+
+// Tiles of row tiles [0, qt) of one (sequence, vh).
+template <int BK>
+__device__ __forceinline__ long long tiles_before(const AttnArgs& a, const Seq& s, int qt) {
+  if (qt <= 0) return 0;
+  if (a.tree != nullptr) return static_cast<long long>(qt) * tiles_of<BK>(s.L);
+  const int all = row_tiles(a, s);
+  long long sum = 0;
+  int whole = qt;
+  if (qt == all) {  // the last row tile may be short
+    sum = tiles_of<BK>(keys_of_tile(a, s, all - 1));
+    whole = all - 1;
+  }
+  // row tile i ends at key base + (i + 1) tq; those that end at or before key 0 still take a tile
+  const long long base = static_cast<long long>(s.L) - s.n;
+  long long none = 0;
+  if (base + a.tq <= 0) none = min(static_cast<long long>(whole), -base / a.tq);
+  sum += none;
+  const long long first = base + (none + 1) * a.tq;  // > 0
+  if (whole > none) sum += floor_sum<BK>(whole - none, a.tq, first + BK - 1);
+  return sum;
+}
+
+// Sums of the sequences before each of kPlanThreads runs of consecutive sequences.
+struct PlanShared {
+  long long before[kPlanThreads + 1];
+  long long warp_sum[kPlanThreads / 32];
+};
+
+struct Cursor {
+  int b, vh, qt;         // segment
+  int keys, tiles;       // of the segment
+  int tile;              // current tile inside it
+  long long start;       // first tile of the segment on the line
+  Seq s;
+};
+
+template <int BK>
+__device__ __forceinline__ long long seq_tiles(const AttnArgs& a, const Seq& s) {
+  return tiles_before<BK>(a, s, row_tiles(a, s)) * (a.c.Hkv * a.nsub);
+}
+
+// Every thread of the CTA calls it; the first kPlanThreads do the work.  Returns W.
+template <int BK>
+__device__ long long plan_build(const AttnArgs& a, PlanShared* sh) {
+  const int per = (a.B + kPlanThreads - 1) / kPlanThreads;
+  const int t = threadIdx.x;
+  long long v = 0, inc = 0;
+  if (t < kPlanThreads) {
+    for (int b = t * per; b < min(a.B, (t + 1) * per); ++b) v += seq_tiles<BK>(a, seq_at(a, b));
+    inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+      if ((t & 31) >= o) inc += up;
+    }
+    if ((t & 31) == 31) sh->warp_sum[t >> 5] = inc;
+  }
+  __syncthreads();
+  if (t < kPlanThreads) {
+    long long add = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 32; ++w)
+      if (w < (t >> 5)) add += sh->warp_sum[w];
+    sh->before[t] = add + inc - v;
+    if (t == kPlanThreads - 1) sh->before[kPlanThreads] = add + inc;
+  }
+  __syncthreads();
+  return sh->before[kPlanThreads];
+}
+
+// Position of tile w of the line (0 <= w < W).  Uniform over the CTA.
+template <int BK>
+__device__ Cursor plan_locate(const AttnArgs& a, const PlanShared* sh, long long w) {
+  int lo = 0, hi = kPlanThreads;  // the last run that starts at or before w
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (sh->before[mid] <= w) lo = mid;
+    else hi = mid;
+  }
+  const int per = (a.B + kPlanThreads - 1) / kPlanThreads;
+  long long at = sh->before[lo];
+  Cursor c;
+  c.b = lo * per;
+  while (true) {  // w < W, so a sequence that holds it comes before B
+    c.s = seq_at(a, c.b);
+    const long long here = seq_tiles<BK>(a, c.s);
+    if (w < at + here || c.b + 1 >= a.B) break;
+    at += here;
+    ++c.b;
+  }
+  const int qts = row_tiles(a, c.s);
+  const long long per_head = max(1ll, tiles_before<BK>(a, c.s, qts));
+  c.vh = static_cast<int>((w - at) / per_head);
+  at += c.vh * per_head;
+  int l = 0, h = qts;
+  while (h - l > 1) {
+    const int mid = (l + h) / 2;
+    if (at + tiles_before<BK>(a, c.s, mid) <= w) l = mid;
+    else h = mid;
+  }
+  c.qt = l;
+  c.start = at + tiles_before<BK>(a, c.s, l);
+  c.keys = keys_of_tile(a, c.s, l);
+  c.tiles = tiles_of<BK>(c.keys);
+  c.tile = static_cast<int>(w - c.start);
+  return c;
+}
+
+// The segment after c's (only called while one exists).
+template <int BK>
+__device__ __forceinline__ void plan_next(const AttnArgs& a, Cursor& c) {
+  c.start += c.tiles;
+  c.tile = 0;
+  if (++c.qt >= row_tiles(a, c.s)) {
+    c.qt = 0;
+    if (++c.vh >= a.c.Hkv * a.nsub) {
+      c.vh = 0;
+      do {
+        ++c.b;
+        c.s = seq_at(a, min(c.b, a.B - 1));
+      } while (c.s.n == 0 && c.b + 1 < a.B);
+    }
+  }
+  c.keys = keys_of_tile(a, c.s, c.qt);
+  c.tiles = tiles_of<BK>(c.keys);
+}
+
+// CTAs that get work: no share below min_tiles while that leaves CTAs idle.
+__device__ __forceinline__ int plan_ctas(const AttnArgs& a, long long W, int grid) {
+  const long long most = (W + a.min_tiles - 1) / a.min_tiles;
+  return static_cast<int>(min(static_cast<long long>(grid), max(1ll, most)));
+}
+__device__ __forceinline__ long long share_begin(long long W, int G, int c) { return W * c / G; }
+__device__ __forceinline__ int share_owner(long long W, int G, long long w) {
+  return static_cast<int>(((w + 1) * G - 1) / W);
+}
+
+}  // namespace smb

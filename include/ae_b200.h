@@ -360,6 +360,77 @@ typedef struct smb_timers {
 } smb_timers_t;
 SMB_API int smb_moe_read_timers(const void* ws, size_t ws_bytes, int reset, smb_timers_t* out, smb_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Paged key/value cache: the other half of a verify step's layer (rotary positions, cache
+ * write, attention over the cache under the draft tree's mask).  The reference runs it through
+ * MHATokenToKVPool (specmoe/backend/memory.py) and its Triton and CPU attention backends
+ * (specmoe/layers/attention_backend/).
+ *
+ * One layer's cache is two arrays of rows [num_pages][kv_heads][page_size] (keys and values,
+ * the same shape and strides; strides in bytes, multiples of 16, so that token-major pools
+ * [tokens][heads][head_dim] are described as well).  A token's slot is page * page_size +
+ * place.  bits = 16: a row is head_dim values of `dtype`.  bits = 4: a row is
+ * smb_kv4_row_bytes(head_dim) bytes: head_dim / 2 bytes of codes (dim 2i in the low nibble of
+ * byte i), then a (scale, zero) pair of `dtype` for each 32 dims, then padding to 16 bytes;
+ * a value is scale * code + zero.
+ * Limits: head_dim 64, 128 or 256; page_size a power of two up to 65536; query heads a multiple
+ * of kv_heads, at most 1024; tokens x query heads below 2^31; tensors 16-byte aligned. */
+typedef struct smb_paged_cache {
+  void* k;
+  void* v;
+  int64_t num_pages;
+  int64_t page_stride, head_stride, token_stride; /* bytes */
+  int kv_heads, page_size, head_dim, bits;
+} smb_paged_cache_t;
+
+/* Bytes of one row of a 4-bit cache (SMB_ERR_SHAPE for an unsupported head size). */
+SMB_API int smb_kv4_row_bytes(int head_dim);
+
+/* New tokens into the cache: RMS norm of every query and key head with q_norm / k_norm
+ * [head_dim] (NULL: none), rotary positions on the first `rot` dims of queries and keys
+ * (rot a multiple of 16, 0: none; pairs (i, i + rot/2), or (2i, 2i + 1) when `interleaved`;
+ * angle = positions[t] * inv_freq[i] in 64 bits, cos and sin times rope_scale), then queries to
+ * q_out [N, Hq, head_dim] and keys and values to the rows of slots[t] (specmoe/models/mixtral.py:
+ * 118-224 rotates and caches in separate kernels).  strides: host array of six, in elements:
+ * token and head stride of q, k and v (multiples of 8; head_dim is contiguous).  A negative slot
+ * is not written; a slot past the cache is not written and recorded as SMB_ERR_BAD_PAGE's device
+ * code in *status (device int, NULL: not recorded).  The slots of a call have to be distinct. */
+SMB_API int smb_kv_append(const smb_paged_cache_t* cache, const void* q, const void* k, const void* v,
+                          const int64_t* strides, int dtype, int N, int Hq, const int64_t* slots,
+                          const int64_t* positions, const double* inv_freq, int rot, int interleaved,
+                          float rope_scale, const void* q_norm, const void* k_norm, float eps, void* q_out,
+                          int* status, smb_stream_t stream);
+
+/* Rows of one 4-bit array (keys or values) as 16-bit values: out [M, kv_heads, head_dim] of `dtype`
+ * for slots [M].  A slot outside the cache reads as zeros. */
+SMB_API int smb_kv4_read(const void* cache, int64_t num_pages, int kv_heads, int page_size, int head_dim,
+                         int64_t page_stride, int64_t head_stride, int64_t token_stride, int dtype,
+                         const int64_t* slots, int M, void* out, smb_stream_t stream);
+
+/* Bytes of workspace one smb_paged_attention call needs (0 for invalid sizes).  It needs no
+ * initialisation and holds nothing between calls. */
+SMB_API size_t smb_paged_attention_workspace_bytes(int N, int B, int Hq, int Hkv, int head_dim, int bits);
+
+/* Attention of the new tokens of B sequences over their cached keys and values.  Sequence b owns
+ * the rows q_starts[b] .. q_starts[b+1]-1 of q [N, Hq, head_dim] (its n_b newest tokens, already in
+ * the cache) and the keys 0 .. kv_lens[b]-1, key j in place j % page_size of page
+ * block_table[b][j / page_size].  With P = kv_lens[b] - n_b, its token i sees key j if j <= P + i;
+ * or, given `tree` [N][tree_words] of 32 bits each, if j < P or bit j - P of its words is set (draft
+ * trees: ancestors and itself; bits beyond the words read as 0).  out = softmax(scale * q k) v,
+ * lse [N, Hq] (optional) = the natural log of the softmax's sum; a token that sees no key gets 0 and
+ * -inf.  Rows of q that belong to no sequence leave out and lse as they were.  Lengths are read on the
+ * device: kv_lens is cut to max_pages * page_size, q_starts to [0, N]; keys of a page outside
+ * [0, num_pages) are left out and recorded in *status (device int, optional).
+ * (specmoe/layers/attention_backend/triton_backend.py, cpu_backend.py; the lse is what joins a
+ * result with another part of the context, as the reference joins its CPU and GPU parts.) */
+SMB_API int smb_paged_attention(const smb_paged_cache_t* cache, const void* q, int64_t q_token_stride,
+                                int64_t q_head_stride, int dtype, int N, int Hq, int B,
+                                const int32_t* block_table, int64_t table_stride, int max_pages,
+                                const int32_t* kv_lens, const int32_t* q_starts, const int32_t* tree,
+                                int64_t tree_stride, int tree_words, float scale, void* out,
+                                int64_t out_token_stride, int64_t out_head_stride, float* lse, int* status,
+                                void* ws, size_t ws_bytes, smb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
