@@ -32,19 +32,11 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "paged_math.cuh"
 #include "paged_plan.cuh"
 
 namespace smb {
 namespace {
-
-constexpr float kLn2 = 0.69314718055994530942f;
-constexpr float kNegInf = -__builtin_huge_valf();
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool fill) {
   const int n = fill ? 16 : 0;
@@ -66,70 +58,6 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
                : "memory");
-}
-
-template <typename T>
-struct Half2;
-template <>
-struct Half2<__nv_bfloat16> {
-  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-  // 16 + nibble e (and e + 4) of w: ulp of 16.0 is 2^-3, so the nibble goes to mantissa bits 3-6
-  static constexpr uint32_t kMask = 0x00780078u, kBase = 0x41804180u;
-  static constexpr int kUp = 3;
-  static __device__ __forceinline__ uint32_t dequant(uint32_t v, uint32_t s2, uint32_t z2) {
-    const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&v);
-    const uint32_t base = kBase;
-    const __nv_bfloat162 d = __hsub2(x, *reinterpret_cast<const __nv_bfloat162*>(&base));
-    const __nv_bfloat162 r = __hfma2(d, *reinterpret_cast<const __nv_bfloat162*>(&s2), *reinterpret_cast<const __nv_bfloat162*>(&z2));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  static __device__ __forceinline__ float lo(uint32_t v) { return __uint_as_float(v << 16); }
-  static __device__ __forceinline__ float hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
-  static __device__ __forceinline__ bool nonfinite(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }
-};
-template <>
-struct Half2<__half> {
-  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-  // ulp of 16.0 is 2^-6: mantissa bits 6-9
-  static constexpr uint32_t kMask = 0x03C003C0u, kBase = 0x4C004C00u;
-  static constexpr int kUp = 6;
-  static __device__ __forceinline__ uint32_t dequant(uint32_t v, uint32_t s2, uint32_t z2) {
-    const __half2 x = *reinterpret_cast<const __half2*>(&v);
-    const uint32_t base = kBase;
-    const __half2 d = __hsub2(x, *reinterpret_cast<const __half2*>(&base));
-    const __half2 r = __hfma2(d, *reinterpret_cast<const __half2*>(&s2), *reinterpret_cast<const __half2*>(&z2));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  static __device__ __forceinline__ float2 both(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-  static __device__ __forceinline__ float lo(uint32_t v) { return both(v).x; }
-  static __device__ __forceinline__ float hi(uint32_t v) { return both(v).y; }
-  static __device__ __forceinline__ bool nonfinite(uint32_t h) { return (h & 0x7c00u) == 0x7c00u; }
-};
-
-// Nibbles e and e + 4 of w as 16 + code, one in each half.
-template <typename T, int E>
-__device__ __forceinline__ uint32_t nib(uint32_t w) {
-  constexpr int sh = Half2<T>::kUp - 4 * E;
-  uint32_t v;
-  if constexpr (sh >= 0) v = w << sh;
-  else v = w >> (-sh);
-  return (v & Half2<T>::kMask) | Half2<T>::kBase;
 }
 
 template <int D, int MT, bool BITS4>

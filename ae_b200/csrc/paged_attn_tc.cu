@@ -1,0 +1,703 @@
+// Attention of many query rows over a paged 16-bit cache on the 5th-generation tensor cores:
+// draft trees (a few dozen tokens x the query heads of a key head) and prefill chunks.
+//
+//   S = Q K^T  (128 rows x 128 keys, fp32 in TMEM),  P = 2^(scale log2(e) S - m),  O += P V
+//
+// with a running maximum m and sum per row.  A row of S lies in one TMEM lane, so a softmax
+// thread owns a row: maximum and sum need no exchange between threads.  P goes back into S's TMEM
+// columns in the 16-bit type and is the A operand of the second product from there; V is its B
+// operand as it lies in memory (keys x dims, "MN-major"), so nothing is transposed.
+//
+// Two streams of 128 rows keep the tensor pipe and the exponentials busy at once: while the four
+// warps of one stream work on their S, the pipe runs the other stream's products.
+//  - DUAL (more than 128 rows for a key head): the streams are two row tiles over the same keys, each
+//    K and V tile is read once for 256 rows.  Bound by arithmetic: per 128 keys and stream 512 clocks
+//    of tensor pipe for each product and 128 exponentials per lane group, 1024 clocks on the
+//    special-function units.
+//  - otherwise the streams take the even and the odd key tiles of the same 128 rows and are added at
+//    the end.  Bound by memory at the sizes of a verify step: a 64 KB tile takes an SM's share of HBM
+//    about 2800 clocks, twice what its products and exponentials take.
+//
+// Keys and values come by TMA, one box per page (its rows of one head) and 64 dims, into a ring of
+// five 128-row slots with the 128-byte swizzle.  Keys past the end and pages outside the cache are
+// boxes at a page coordinate past the tensor: TMA writes zeros there, and the mask drops them.  Rows
+// behind the last key inside a page, and new tokens that a row may not see, may hold anything: where
+// a mask cuts a tile, the softmax warps look through V in shared memory before the product, take
+// non-finite values out, and the rows that do see them get them added from memory at the end.
+//
+// Every wait is bounded.  After a failed one all roles run on to the end of their loops without
+// waiting (their results are void, the status says so), so barriers between warps still match.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+#include "host.h"
+#include "kernels.h"
+#include "paged_math.cuh"
+#include "paged_plan.cuh"
+
+namespace smb {
+namespace {
+
+constexpr int kTBK = 128;       // keys of a tile
+constexpr int kTSlots = 5;      // ring slots
+constexpr int kTThreads = 384;  // warp 0 TMA, warp 1 MMA, warp 2 TMEM, warp 3 idle, warps 4-7 / 8-11 softmax
+constexpr int kTOkRing = 8;     // tiles whose page masks are kept: the ring lets K run at most 5 tiles ahead
+enum : int { kFixValues = 1, kFixBadPage = 2 };  // this CTA met non-finite values behind a mask / bad pages
+
+template <int D, bool DUAL>
+struct TcCfg {
+  static constexpr int R = DUAL ? 256 : 128;
+  static constexpr int TILE = kTBK * D * 2;                 // bytes of a K or V tile, and of 128 rows of Q
+  static constexpr int Q = (DUAL ? 2 : 1) * TILE;
+  static constexpr int MERGE = DUAL ? 0 : 128 * 32 * 4;     // 32 columns of the second stream's output
+  static constexpr int SMEM = Q + kTSlots * TILE + MERGE + 1024;
+};
+
+// TMEM columns: S of the streams at 0 and 128 (P in their first 64), O at 256 and 384.
+constexpr uint32_t kTmemS = 0, kTmemO = 256;
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+          "r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// D[tmem] (+)= A[tmem] * B[smem], kind::f16.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Descriptor of an MN-major operand (V: rows of 64 dims = 128 bytes, one row per key) in the 128-byte
+// swizzle: 8-key groups 1024 bytes apart (stride offset), the next 64 dims `half` bytes on (leading
+// offset).
+__device__ __forceinline__ uint64_t desc_mnmajor_sw128(uint32_t addr, uint32_t half) {
+  uint64_t d = desc_kmajor_sw128(addr) & ~(0x3FFFull << 16);
+  return d | static_cast<uint64_t>(half >> 4) << 16;
+}
+constexpr uint32_t kIdescBMn = 1u << 16;  // B is MN-major
+
+#define SMB_R4(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
+#define SMB_R16(v, i) SMB_R4(v, i), SMB_R4(v, i + 4), SMB_R4(v, i + 8), SMB_R4(v, i + 12)
+#define SMB_P4(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3])
+#define SMB_P16(v, i) SMB_P4(v, i), SMB_P4(v, i + 4), SMB_P4(v, i + 8), SMB_P4(v, i + 12)
+#define SMB_I4(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3])
+#define SMB_I16(v, i) SMB_I4(v, i), SMB_I4(v, i + 4), SMB_I4(v, i + 8), SMB_I4(v, i + 12)
+
+// 32 columns of this thread's lane, issued only; tmem_ld_done(v) before v is used.
+__device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : SMB_R16(v, 0), SMB_R16(v, 16)
+      : "r"(taddr)
+      : "memory");
+}
+// Waits for every issued load; the values pass through so that no use moves before the wait.
+__device__ __forceinline__ void tmem_ld_done(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : SMB_P16(v, 0), SMB_P16(v, 16) : : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      SMB_I16(v, 0), SMB_I16(v, 16)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void named_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+
+// The segments of this CTA's share, walked alike by every role.
+struct Walk {
+  Cursor cur;
+  long long w, w_hi;
+  int t0, t1;
+  __device__ __forceinline__ void open() {
+    t0 = cur.tile;
+    t1 = static_cast<int>(min(static_cast<long long>(cur.tiles), cur.tile + (w_hi - w)));
+  }
+  __device__ __forceinline__ bool next(const AttnArgs& a) {
+    w += t1 - t0;
+    if (w >= w_hi) return false;
+    plan_next<kTBK>(a, cur);
+    open();
+    return true;
+  }
+};
+
+template <int D, bool DUAL, typename T>
+__global__ void __launch_bounds__(kTThreads, 1)
+    paged_attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v) {
+  using C = TcCfg<D, DUAL>;
+  using H = Half2<T>;
+  constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int R = C::R, TILE = C::TILE;
+  constexpr uint32_t HALF = kTBK * 128;  // bytes of 64 dims of a tile
+  extern __shared__ uint8_t dyn_smem[];
+  __shared__ PlanShared s_plan;
+  __shared__ uint64_t full_bar[kTSlots], empty_bar[kTSlots], s_bar[2], p_bar[2], o_bar[2], q_bar[2], drain_bar;
+  __shared__ uint32_t s_tmem, s_pages[kTOkRing];
+  __shared__ int s_abort, s_fix;
+  __shared__ float2 s_ml[DUAL ? 1 : 128];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t raw = smem_u32(dyn_smem);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* sm = dyn_smem + (base - raw);
+  const uint32_t q_s = base, ring_s = base + C::Q;
+
+  if (tid == 0) {
+    s_abort = 0;
+    s_fix = 0;
+    for (int i = 0; i < kTSlots; ++i) {
+      mbar_init(&full_bar[i], 1);
+      mbar_init(&empty_bar[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_bar[i], 1);
+      mbar_init(&p_bar[i], 128);
+      mbar_init(&o_bar[i], 1);
+      mbar_init(&q_bar[i], 128);
+    }
+    mbar_init(&drain_bar, 1);
+    fence_mbarrier_init();
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+  }
+  if (warp == 2) {
+    tmem_alloc(&s_tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+
+  pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  const long long W = plan_build<kTBK>(a, &s_plan);
+  const int Gc = plan_ctas(a, W, gridDim.x);
+  const int cta = blockIdx.x;
+  const long long w_lo = W > 0 && cta < Gc ? share_begin(W, Gc, cta) : 0;
+  const long long w_hi = W > 0 && cta < Gc ? share_begin(W, Gc, cta + 1) : 0;
+  int* status = a.status;
+  volatile int* abort_flag = &s_abort;
+
+  if (w_lo < w_hi) {
+    Walk k;
+    k.cur = plan_locate<kTBK>(a, &s_plan, w_lo);
+    k.w = w_lo;
+    k.w_hi = w_hi;
+    k.open();
+
+    if (warp < 4) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+      if (warp == 0) {
+        // ---------------------------------------------------------------- TMA
+        const int psb = min(1 << a.c.page_shift, kTBK);  // rows of a box
+        const int pages = kTBK / psb, boxes = pages * (D / 64);
+        const int page_mask = (1 << a.c.page_shift) - 1;
+        int it = 0, tc = 0;
+        // a tile's boxes, one per page and 64 dims (at most 32: a lane issues one)
+        auto load = [&](const CUtensorMap* map, int t, bool is_k) {
+          const int slot = it % kTSlots;
+          const int p = lane % pages, j = t * kTBK + p * psb;
+          const bool in = j < k.cur.keys;
+          const int page = in ? a.table[k.cur.b * a.table_stride + (j >> a.c.page_shift)] : -1;
+          const bool good = page >= 0 && page < a.c.num_pages;
+          const uint32_t bad = __ballot_sync(0xffffffffu, in && lane < pages && !good);
+          if (is_k) {
+            if (lane == 0) {
+              s_pages[tc % kTOkRing] = ~bad;
+              if (bad != 0) {
+                record_status(status, kDevBadPage);
+                atomicOr(&s_fix, kFixBadPage);
+              }
+            }
+            ++tc;
+          }
+          mbar_wait(&empty_bar[slot], ((it / kTSlots) & 1) ^ 1, status, abort_flag);
+          if (lane == 0) mbar_arrive_expect_tx(&full_bar[slot], TILE);
+          __syncwarp();
+          if (lane < boxes) {
+            const int h = lane / pages;
+            tma_load_4d(ring_s + slot * TILE + h * HALF + p * psb * 128, map, &full_bar[slot], h * 64, j & page_mask,
+                        k.cur.vh / a.nsub, good ? page : static_cast<int>(a.c.num_pages));
+          }
+          ++it;
+        };
+        do {
+          const int n = k.t1 - k.t0;
+          if constexpr (DUAL) {
+            for (int t = k.t0; t < k.t1; ++t) {
+              load(&tm_k, t, true);
+              load(&tm_v, t, false);
+            }
+          } else {
+            load(&tm_k, k.t0, true);
+            if (n > 1) load(&tm_k, k.t0 + 1, true);
+            for (int i = 0; i < n; ++i) {
+              load(&tm_v, k.t0 + i, false);
+              if (i + 2 < n) load(&tm_k, k.t0 + i + 2, true);
+            }
+          }
+        } while (k.next(a));
+        // the copies into every slot have landed before the CTA may end
+        for (int i = max(0, it - kTSlots); i < it; ++i)
+          mbar_wait(&full_bar[i % kTSlots], (i / kTSlots) & 1, status, nullptr);
+      } else if (warp == 1 && lane == 0) {
+        // ---------------------------------------------------------------- MMA
+        constexpr uint32_t idesc_s = idesc_f16(kBF16, 128, kTBK);
+        constexpr uint32_t idesc_o = idesc_f16(kBF16, 128, D) | kIdescBMn;
+        int it = 0, np[2] = {0, 0}, seg = 0;
+        auto wait_full = [&](int i) {
+          mbar_wait(&full_bar[i % kTSlots], (i / kTSlots) & 1, status, abort_flag);
+          tc_fence_after();
+        };
+        auto qk = [&](int i, int s) {  // S_s = Q_s K^T, K in the slot of step i
+          const uint32_t ks = ring_s + (i % kTSlots) * TILE, qs = q_s + (DUAL ? s * TILE : 0);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk / 4) * HALF + (kk % 4) * 32;
+            umma_f16(tmem + kTmemS + s * 128, desc_kmajor_sw128(qs + off), desc_kmajor_sw128(ks + off), idesc_s, kk > 0);
+          }
+        };
+        auto pv = [&](int i, int s, bool first) {  // O_s (+)= P_s V
+          const uint32_t vs = ring_s + (i % kTSlots) * TILE;
+#pragma unroll
+          for (int kk = 0; kk < kTBK / 16; ++kk)
+            umma_f16_ts(tmem + kTmemO + s * 128, tmem + kTmemS + s * 128 + kk * 8,
+                        desc_mnmajor_sw128(vs + kk * 2048, HALF), idesc_o, !(first && kk == 0));
+        };
+        auto wait_p = [&](int s) {
+          mbar_wait(&p_bar[s], np[s] & 1, status, abort_flag);
+          ++np[s];
+          tc_fence_after();
+        };
+        do {
+          const int n = k.t1 - k.t0;
+          mbar_wait(&q_bar[0], seg & 1, status, abort_flag);
+          mbar_wait(&q_bar[1], seg & 1, status, abort_flag);
+          tc_fence_after();
+          ++seg;
+          if constexpr (DUAL) {
+            int kslot = it++;
+            wait_full(kslot);
+            qk(kslot, 0);
+            umma_commit(&s_bar[0]);
+            qk(kslot, 1);
+            umma_commit(&s_bar[1]);
+            umma_commit(&empty_bar[kslot % kTSlots]);
+            for (int t = 0; t < n; ++t) {
+              const bool more = t + 1 < n;
+              const int vslot = it++;
+              if (more) kslot = it++;
+              wait_full(vslot);
+              wait_p(0);
+              pv(vslot, 0, t == 0);
+              if (more) {
+                wait_full(kslot);
+                qk(kslot, 0);
+                umma_commit(&s_bar[0]);
+              } else {
+                umma_commit(&o_bar[0]);
+              }
+              wait_p(1);
+              pv(vslot, 1, t == 0);
+              umma_commit(&empty_bar[vslot % kTSlots]);
+              if (more) {
+                qk(kslot, 1);
+                umma_commit(&s_bar[1]);
+                umma_commit(&empty_bar[kslot % kTSlots]);
+              } else {
+                umma_commit(&o_bar[1]);
+              }
+            }
+          } else {
+            for (int s = 0; s < min(n, 2); ++s) {
+              wait_full(it);
+              qk(it, s);
+              umma_commit(&empty_bar[it % kTSlots]);
+              umma_commit(&s_bar[s]);
+              ++it;
+            }
+            for (int t = 0; t < n; ++t) {
+              const int s = t & 1;
+              wait_full(it);
+              wait_p(s);
+              pv(it, s, t < 2);
+              umma_commit(&empty_bar[it % kTSlots]);
+              ++it;
+              if (t + 2 < n) {
+                wait_full(it);
+                qk(it, s);
+                umma_commit(&empty_bar[it % kTSlots]);
+                umma_commit(&s_bar[s]);
+                ++it;
+              } else {
+                umma_commit(&o_bar[s]);
+              }
+            }
+          }
+        } while (k.next(a));
+        umma_commit(&drain_bar);
+        mbar_wait(&drain_bar, 0, status, nullptr);
+      }
+    } else {
+      // ------------------------------------------------------------------ softmax and output
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+      const int s = (warp - 4) >> 2;                  // stream
+      const int row = (warp & 3) * 32 + lane;         // TMEM lane
+      const int r = DUAL ? s * 128 + row : row;       // row of the row tile
+      const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+      const uint32_t t_s = t_lane + kTmemS + s * 128, t_o = t_lane + kTmemO + s * 128;
+      int it = 0, tc = 0, ns = 0, no = 0;
+      const int tok_r = r / a.gs, sub_r = r % a.gs;
+      do {
+        const int n = k.t1 - k.t0;
+        const Cursor& cur = k.cur;
+        const int kvh = cur.vh / a.nsub, sub = cur.vh % a.nsub;
+        const int heads = min(a.gs, a.g - sub * a.gs);
+        const int tok0 = cur.qt * a.tq, toks = min(a.tq, cur.s.n - tok0);
+        const int prefix = cur.s.L - cur.s.n;
+        const bool row_ok = tok_r < toks && sub_r < heads;
+        const int open = a.tree != nullptr ? prefix : prefix + tok0 + 1;  // first key some row may not see
+        const long long tok = cur.s.s0 + tok0 + tok_r;
+        const int head = kvh * a.g + sub * a.gs + sub_r;
+        // ---- Q: 16-byte chunks of a row, swizzled as TMA would write them
+        {
+          const int rq = DUAL ? r : (tid - 128) & 127;
+          const int tokq = rq / a.gs, subq = rq % a.gs;
+          const bool okq = tokq < toks && subq < heads;
+          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (cur.s.s0 + tok0 + tokq) * a.q_ts +
+                                                            (kvh * a.g + sub * a.gs + subq) * a.q_hs);
+          constexpr int CH = D / 8;
+          const int c0 = DUAL ? 0 : s * (CH / 2), c1 = DUAL ? CH : c0 + CH / 2;
+          const int rr = rq & 127;
+          uint8_t* dst = sm + (DUAL ? s * TILE : 0) + rr * 128;
+#pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            if (c < c0 || c >= c1) continue;
+            const uint4 v = okq ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(dst + (c >> 3) * HALF + (((c & 7) ^ (rr & 7)) << 4)) = v;
+          }
+          fence_async_proxy();
+          mbar_arrive(&q_bar[s]);
+        }
+        float m = kNegInf, l = 0.f;
+        auto visible = [&](int j) {  // this row, key j
+          if (!row_ok || j >= cur.keys) return false;
+          const int lj = j - prefix;
+          if (a.tree == nullptr) return lj <= tok0 + tok_r;
+          if (lj < 0) return true;
+          return (lj >> 5) < a.tree_words &&
+                 ((static_cast<uint32_t>(a.tree[tok * a.tree_stride + (lj >> 5)]) >> (lj & 31)) & 1u) != 0;
+        };
+        for (int i = DUAL ? 0 : s; i < n; i += DUAL ? 1 : 2) {
+          const int j0 = (k.t0 + i) * kTBK;
+          mbar_wait(&s_bar[s], ns & 1, status, abort_flag);
+          tc_fence_after();
+          const uint32_t pages_ok = s_pages[(tc + i) % kTOkRing];
+          const bool masked = j0 + kTBK > open || j0 + kTBK > cur.keys || pages_ok != 0xffffffffu;
+          uint32_t x[4][32];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) tmem_ld32_issue(t_s + q * 32, x[q]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) tmem_ld_done(x[q]);
+          if (masked) {
+            const int psb = min(1 << a.c.page_shift, kTBK);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int jq = j0 + q * 32;
+              uint32_t see = 0;  // bit e: this row sees key jq + e
+              const int left = min(32, cur.keys - jq);
+              if (row_ok && left > 0) {
+                see = left == 32 ? 0xffffffffu : (1u << left) - 1u;
+                const int lj = jq - prefix;
+                if (a.tree == nullptr) {
+                  const int c = tok0 + tok_r - lj + 1;
+                  see &= c >= 32 ? 0xffffffffu : c <= 0 ? 0u : (1u << c) - 1u;
+                } else if (lj > -32) {
+                  const int w0 = lj >> 5, sh = lj & 31;  // (floor: lj may be negative)
+                  const int* words = a.tree + tok * a.tree_stride;
+                  const uint32_t lo = w0 < 0 ? 0xffffffffu : w0 < a.tree_words ? static_cast<uint32_t>(words[w0]) : 0u;
+                  const uint32_t hi = w0 + 1 < a.tree_words ? static_cast<uint32_t>(words[w0 + 1]) : 0u;
+                  see &= __funnelshift_r(lo, hi, sh);
+                }
+                if (pages_ok != 0xffffffffu) {
+                  for (int e = 0; e < 32; ++e)
+                    if (!((pages_ok >> ((q * 32 + e) / psb)) & 1u)) see &= ~(1u << e);
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!((see >> e) & 1u)) x[q][e] = __float_as_uint(kNegInf);
+            }
+            // V: what no mask stops from entering the product has to be finite
+            const int vstep = it + (DUAL ? 2 * i + 1 : i + min(i + 2, n));
+            mbar_wait(&full_bar[vstep % kTSlots], (vstep / kTSlots) & 1, status, abort_flag);
+            uint8_t* vp = sm + C::Q + (vstep % kTSlots) * TILE + row * 128;
+            const bool dead = j0 + row >= cur.keys;  // a row behind the keys
+            bool bad = false;
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+              uint4* p = reinterpret_cast<uint4*>(vp + (c >> 3) * HALF + ((c & 7) << 4));
+              uint4 v = *p;
+              uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+              bool hit = false;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (H::nonfinite(u[e] & 0xffffu)) u[e] &= 0xffff0000u, hit = true;
+                if (H::nonfinite(u[e] >> 16)) u[e] &= 0xffffu, hit = true;
+              }
+              if (hit) {
+                bad = true;
+                if (!dead) atomicOr(&s_fix, kFixValues);  // before the value goes
+                __threadfence_block();
+                *p = v;
+              }
+            }
+            if (bad) fence_async_proxy();
+          }
+
+          float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(x[q][e]));
+          const float tmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+          // a row is rescaled only when its maximum grew by more than 8 (p stays below 2^8)
+          const bool grew = tmax > m + 8.f;
+          if (__any_sync(0xffffffffu, grew)) {
+            const float now = grew ? tmax : m;
+            const float f = m == kNegInf ? 0.f : exp2_fast(m - now);
+            m = now;
+            l *= f;
+            if (i >= (DUAL ? 1 : 2)) {
+              // (this stream's last product is complete: it was issued before the S just waited for)
+#pragma unroll
+              for (int q = 0; q < D / 32; ++q) {
+                uint32_t o[32];
+                tmem_ld32_issue(t_o + q * 32, o);
+                tmem_ld_done(o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st32(t_o + q * 32, o);
+              }
+              tmem_st_done();
+            }
+          }
+          const float mm = m == kNegInf ? 0.f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            uint32_t p[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float v0 = exp2_fast(fmaf(__uint_as_float(x[2 * q + e / 16][(e % 16) * 2]), a.scale_log2, -mm));
+              const float v1 = exp2_fast(fmaf(__uint_as_float(x[2 * q + e / 16][(e % 16) * 2 + 1]), a.scale_log2, -mm));
+              sum[e & 1] += v0;
+              sum[2 + (e & 1)] += v1;
+              p[e] = H::pack(v0, v1);
+            }
+            tmem_st32(t_s + q * 32, p);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st_done();
+          tc_fence_before();
+          mbar_arrive(&p_bar[s]);
+          ++ns;
+        }
+
+        // ---- output
+        const bool mine = DUAL || n > s;  // this stream had a tile
+        if (mine) {
+          mbar_wait(&o_bar[s], no & 1, status, abort_flag);
+          ++no;
+          tc_fence_after();
+        }
+        const bool whole = k.t0 == 0 && k.t1 == cur.tiles;
+        const long long slot = 2ll * cta + (cur.start > w_lo ? 1 : 0);
+        float f0 = 1.f, f1 = 0.f;
+        if constexpr (!DUAL) {
+          if (s == 1) s_ml[row] = make_float2(m, l);
+          named_sync(1, 256);
+          if (s == 0) {
+            const float2 o = s_ml[row];
+            const float both = fmaxf(m, o.x);
+            f0 = m == kNegInf ? 1.f : exp2_fast(m - both);
+            f1 = o.x == kNegInf ? 1.f : exp2_fast(o.x - both);
+            l = l * f0 + o.y * f1;
+            m = both;
+          }
+        }
+        const int fix = *reinterpret_cast<volatile int*>(&s_fix);
+        float inv = 1.f;
+        if (whole) inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t o[32];
+          __syncwarp();
+          if (mine) {
+            tmem_ld32_issue(t_o + q * 32, o);
+            tmem_ld_done(o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0u;
+          }
+          if ((fix & kFixValues) && row_ok) {
+            // non-finite values that were taken out of this stream's masked tiles, and that this row sees
+            for (int i = DUAL ? 0 : s; i < n; i += DUAL ? 1 : 2) {
+              const int j0 = (k.t0 + i) * kTBK;
+              if (j0 + kTBK <= open && j0 + kTBK <= cur.keys && !(fix & kFixBadPage)) continue;
+              for (int j = j0; j < min(j0 + kTBK, cur.keys); ++j) {
+                if (!visible(j)) continue;
+                const int page = a.table[cur.b * a.table_stride + (j >> a.c.page_shift)];
+                if (page < 0 || page >= a.c.num_pages) continue;
+                const T* v = reinterpret_cast<const T*>(a.c.v + page * a.c.page_stride + kvh * a.c.head_stride +
+                                                        (j & ((1 << a.c.page_shift) - 1)) * a.c.token_stride) + q * 32;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  const float f = to_f32<T>(v[e]);
+                  if (!isfinite(f)) o[e] = __float_as_uint(__uint_as_float(o[e]) + f);
+                }
+              }
+            }
+          }
+          if constexpr (!DUAL) {
+            float* merge = reinterpret_cast<float*>(sm + C::Q + kTSlots * TILE);
+            if (s == 1) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) merge[e * 128 + row] = __uint_as_float(o[e]);
+            }
+            __syncwarp();
+            named_sync(1, 256);
+            if (s == 0) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                o[e] = __float_as_uint(__uint_as_float(o[e]) * f0 + merge[e * 128 + row] * f1);
+            }
+            named_sync(1, 256);  // the next columns go to the same place
+          }
+          if ((DUAL || s == 0) && row_ok) {
+            if (whole) {
+              uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + q * 32);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                uint4 v;
+                v.x = H::pack(__uint_as_float(o[8 * c]) * inv, __uint_as_float(o[8 * c + 1]) * inv);
+                v.y = H::pack(__uint_as_float(o[8 * c + 2]) * inv, __uint_as_float(o[8 * c + 3]) * inv);
+                v.z = H::pack(__uint_as_float(o[8 * c + 4]) * inv, __uint_as_float(o[8 * c + 5]) * inv);
+                v.w = H::pack(__uint_as_float(o[8 * c + 6]) * inv, __uint_as_float(o[8 * c + 7]) * inv);
+                dst[c] = v;
+              }
+            } else {
+              uint4* dst = reinterpret_cast<uint4*>(a.part_o + (slot * R + r) * D + q * 32);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) dst[c] = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+            }
+          }
+        }
+        if ((DUAL || s == 0) && row_ok) {
+          if (!whole) {
+            *reinterpret_cast<float2*>(a.part_ml + (slot * R + r) * 2) = make_float2(m, l);
+          } else if (a.lse != nullptr) {
+            a.lse[tok * (static_cast<long long>(a.c.Hkv) * a.g) + head] = l == 0.f ? kNegInf : (m + log2f(l)) * kLn2;
+          }
+        }
+        tc_fence_before();
+        it += 2 * n;
+        tc += n;
+        __syncwarp();
+        if constexpr (!DUAL) named_sync(1, 256);  // both streams are done with Q and (m, l)
+      } while (k.next(a));
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+template <int D, bool DUAL>
+const void* tc_fn(bool bf16) {
+  return bf16 ? reinterpret_cast<const void*>(paged_attn_tc_kernel<D, DUAL, __nv_bfloat16>)
+              : reinterpret_cast<const void*>(paged_attn_tc_kernel<D, DUAL, __half>);
+}
+
+std::atomic<int> g_smem_seen[8][64];
+
+// Rows [page_size][kv_heads][num_pages] of D 16-bit values; boxes of 64 dims x one page's rows.
+bool encode_cache(CUtensorMap* map, const PagedCacheArgs& c, const void* base, int D, bool bf16) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), 1ull << c.page_shift, static_cast<cuuint64_t>(c.Hkv),
+                              static_cast<cuuint64_t>(c.num_pages)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(c.token_stride), static_cast<cuuint64_t>(c.head_stride),
+                                 static_cast<cuuint64_t>(c.page_stride)};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(std::min(1 << c.page_shift, kTBK)), 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
+            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+bool tc_takes(const PagedCacheArgs& c) {
+  // (strides of dimensions of size 1 mean nothing, but the encoder wants usable ones)
+  const long long most = 1ll << 40;
+  return c.page_shift >= 3 && c.num_pages >= 1 && c.num_pages < 0x7fffffffll && c.token_stride >= 16 &&
+         c.token_stride < most && c.head_stride >= 16 && c.head_stride < most && c.page_stride >= 16 &&
+         c.page_stride < most;
+}
+
+bool plan_attn_tc(int N, int B, int g, int D, bool bits4, int sms, AttnPlan* p) {
+  if (bits4 || D > 128 || g > 128) return false;
+  const long long rows = (static_cast<long long>(N) * g + B - 1) / B;
+  if (rows <= kTcMinRows) return false;
+  p->rows = rows > 128 ? 256 : 128;
+  p->grid = sms;
+  return true;
+}
+
+cudaError_t launch_attn_tc(AttnArgs a, const AttnPlan& p, int D, bool bf16, cudaStream_t stream, bool pdl, bool* fits) {
+  CUtensorMap tk, tv;
+  *fits = encode_cache(&tk, a.c, a.c.k, D, bf16) && encode_cache(&tv, a.c, a.c.v, D, bf16);
+  if (!*fits) return cudaSuccess;
+  const bool dual = p.rows == 256;
+  const void* fn = D == 64 ? (dual ? tc_fn<64, true>(bf16) : tc_fn<64, false>(bf16))
+                           : (dual ? tc_fn<128, true>(bf16) : tc_fn<128, false>(bf16));
+  const int smem = D == 64 ? (dual ? TcCfg<64, true>::SMEM : TcCfg<64, false>::SMEM)
+                           : (dual ? TcCfg<128, true>::SMEM : TcCfg<128, false>::SMEM);
+  cudaError_t err = ensure_dyn_smem(fn, smem, g_smem_seen[(D == 128) * 4 + dual * 2 + bf16], 64);
+  if (err != cudaSuccess) return err;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.grid);
+  cfg.blockDim = dim3(kTThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  void* params[] = {&a, &tk, &tv};
+  err = cudaLaunchKernelExC(&cfg, fn, params);
+  if (err != cudaSuccess) return err;
+  return launch_attn_join(a, p, kTBK, D, bf16, stream, pdl);
+}
+
+}  // namespace smb

@@ -1,4 +1,6 @@
 // C ABI entry points of the paged key/value cache: argument checks and launches.
+#include <algorithm>
+
 #include "../../include/ae_b200.h"
 #include "host.h"
 #include "paged.h"
@@ -151,7 +153,12 @@ size_t smb_paged_attention_workspace_bytes(int N, int B, int Hq, int Hkv, int he
   DeviceInfo di;
   if (device_info(&di) != SMB_OK) return 0;
   if (N == 0 || B == 0) return 256;
-  return attn_ws(plan_attn_mma(N, B, Hq / Hkv, head_dim, bits == 4, di.sms), head_dim);
+  // what either kernel takes at these sizes (which one runs depends on the cache's pages too)
+  const int g = Hq / Hkv;
+  size_t n = attn_ws(plan_attn_mma(N, B, g, head_dim, bits == 4, di.sms), head_dim);
+  AttnPlan p;
+  if (plan_attn_tc(N, B, g, head_dim, bits == 4, di.sms, &p)) n = std::max(n, attn_ws(p, head_dim));
+  return n;
 }
 
 int smb_paged_attention(const smb_paged_cache_t* cache, const void* q, int64_t q_token_stride, int64_t q_head_stride,
@@ -168,6 +175,7 @@ int smb_paged_attention(const smb_paged_cache_t* cache, const void* q, int64_t q
   rc = attn_sizes(N, B, Hq, a.c.Hkv, D, cache->bits);
   if (rc != SMB_OK) return rc;
   if (max_pages < 0 || table_stride < 0 || (tree != nullptr && (tree_words < 1 || tree_stride < 0))) return SMB_ERR_SHAPE;
+  if (!(scale > 0.f) || scale > 1e30f) return SMB_ERR_SHAPE;
   if (N == 0 || B == 0) return SMB_OK;
   if (q == nullptr || out == nullptr || kv_lens == nullptr || q_starts == nullptr || ws == nullptr) return SMB_ERR_NULL;
   if (max_pages > 0 && block_table == nullptr) return SMB_ERR_NULL;
@@ -197,16 +205,27 @@ int smb_paged_attention(const smb_paged_cache_t* cache, const void* q, int64_t q
   a.lse = lse;
   a.status = status;
   const bool bits4 = cache->bits == 4;
-  const AttnPlan p = plan_attn_mma(N, B, a.g, D, bits4, di.sms);
-  if (ws_bytes < attn_ws(p, D)) return SMB_ERR_WORKSPACE;
-  a.gs = a.g < p.rows ? a.g : p.rows;
-  a.nsub = (a.g + a.gs - 1) / a.gs;
-  a.tq = p.rows / a.gs;
-  a.part_o = static_cast<float*>(ws);
-  a.part_ml = a.part_o + static_cast<size_t>(2) * p.grid * p.rows * D;
-  a.min_tiles = 2;
-  return done(launch_attn_mma(a, p, D, dtype == SMB_DTYPE_BF16, bits4, reinterpret_cast<cudaStream_t>(stream),
-                              pdl_enabled()));
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const bool bf16 = dtype == SMB_DTYPE_BF16;
+  AttnPlan p;
+  auto use = [&]() {
+    a.gs = std::min(a.g, p.rows);
+    a.nsub = (a.g + a.gs - 1) / a.gs;
+    a.tq = p.rows / a.gs;
+    a.part_o = static_cast<float*>(ws);
+    a.part_ml = a.part_o + static_cast<size_t>(2) * p.grid * p.rows * D;
+    a.min_tiles = 2;
+    return ws_bytes >= attn_ws(p, D);
+  };
+  if (tc_takes(a.c) && plan_attn_tc(N, B, a.g, D, bits4, di.sms, &p)) {
+    if (!use()) return SMB_ERR_WORKSPACE;
+    bool fits = false;
+    const cudaError_t err = launch_attn_tc(a, p, D, bf16, st, pdl_enabled(), &fits);
+    if (err != cudaSuccess || fits) return done(err);
+  }
+  p = plan_attn_mma(N, B, a.g, D, bits4, di.sms);
+  if (!use()) return SMB_ERR_WORKSPACE;
+  return done(launch_attn_mma(a, p, D, bf16, bits4, st, pdl_enabled()));
 }
 
 }  // extern "C"

@@ -286,7 +286,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``block_table`` int32 [B, max_pages], ``kv_lens`` int32 [B], ``q_starts`` int32 [B + 1].  Without
     ``tree`` the new tokens are causal.  ``tree`` int32 [N, words] (:func:`pack_mask`,
     :func:`tree_words`): token i sees every key before the sequence's new tokens, and new token t
-    where bit t is set.  ``scale`` defaults to head_dim ** -0.5.  ``lse`` float32 [N, Hq], optional:
+    where bit t is set.  ``scale`` (positive) defaults to
+    head_dim ** -0.5.  ``lse`` float32 [N, Hq], optional:
     receives the natural log of each softmax's sum (-inf, with an output of 0, for a token that sees no
     key).  Rows of q behind the last sequence leave ``out`` and ``lse`` as they were.  ``out`` may not
     overlap q.  ``status`` int32 [1] is set to :data:`BAD_PAGE` by a page outside the cache (its keys
@@ -325,12 +326,15 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (N, Hq) or lse.device != dev
                             or not lse.is_contiguous()):
         raise ValueError("lse must be contiguous float32 [N, Hq] on the device of q")
+    scale = float(D ** -0.5 if scale is None else scale)
+    if not 0.0 < scale <= 1e30:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
     word, mine = _status_word(status, dev)
     nbytes = _workspace_bytes(N, B, Hq, cache, dev)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _call(dev, "smb_paged_attention", ctypes.byref(cache), q.data_ptr(), qts, qhs, code, N, Hq, B,
           block_table.data_ptr(), block_table.stride(0) if B > 1 else max_pages, max_pages, lens_p, starts_p, tree_p,
-          tree_stride, words, float(D ** -0.5 if scale is None else scale), out.data_ptr(), ots, ohs,
+          tree_stride, words, scale, out.data_ptr(), ots, ohs,
           None if lse is None else lse.data_ptr(), None if word is None else word.data_ptr(), ws.data_ptr(), nbytes)
     if mine:
         _raise_status("smb_paged_attention", word)

@@ -92,6 +92,14 @@ SHAPES = [
     ([20, 64, 1], [20, 64, 130], 12, 2, 64, 16, True),
     ([33, 5], [170, 2], 3, 3, 256, 32, True),
     ([70, 100], [333, 100], 6, 1, 128, 16, True),
+    # many rows: one and two row tiles of 128 at a time, short and long, pages from 8 to 256
+    ([16, 40, 9], [16, 3000, 500], 8, 2, 64, 8, True),
+    ([64], [5000], 4, 2, 128, 256, False),
+    ([60, 3, 64], [60, 130, 127], 6, 3, 128, 128, False),
+    ([300, 500, 0, 7], [1300, 500, 3, 260], 16, 8, 64, 32, False),
+    ([33] * 40, [33 + 29 * i for i in range(40)], 8, 2, 128, 64, True),
+    ([200], [100], 10, 2, 128, 8, False),
+    ([130, 90], [130, 1000], 96, 1, 64, 16, True),
 ]
 
 
@@ -115,39 +123,42 @@ def test_tree_words_fewer_than_tokens(bits):
     assert bool((out[0] == 0).all()) and bool(torch.isinf(lse[0]).all())
 
 
+@pytest.mark.parametrize("more", [0, 60])
 @pytest.mark.parametrize("bits", [16, 4])
-def test_scale_strides_and_rows_of_no_sequence(bits):
+def test_scale_strides_and_rows_of_no_sequence(bits, more):
     """Another scale; token-major pools; q and out as slices; a table with a row stride; q_starts that
     skip the first rows and end before the last."""
     from ae_b200 import paged
-    d = make_batch([9, 1, 4], [300, 77, 4], 8, 2, 128, 16, BF, bits, False, seed=3)
+    d = make_batch([9 + more, 1, 4], [300, 77, 4], 8, 2, 128, 16, BF, bits, False, seed=3)
+    N = 14 + more
     for name in ("k_cache", "v_cache"):
         c = d[name]
         pool = torch.zeros(c.shape[0], c.shape[2], c.shape[1] + 1, c.shape[3], dtype=c.dtype, device="cuda")
         pool[:, :, :-1] = c.transpose(1, 2)
         d[name] = pool.transpose(1, 2)[:, :-1]
-    wide = torch.randn(14 + 4, 8 + 3, 128, device="cuda").to(BF)
-    wide[2:16, 1:9] = d["q"]
+    wide = torch.randn(N + 4, 8 + 3, 128, device="cuda").to(BF)
+    wide[2:N + 2, 1:9] = d["q"]
     d["q"] = wide[:, 1:9]
     d["q_starts"] += 2
     table = torch.zeros(3, d["block_table"].shape[1] + 5, dtype=torch.int32, device="cuda")
     table[:, :d["block_table"].shape[1]] = d["block_table"]
     d["block_table"] = table[:, :d["block_table"].shape[1]]
-    buf = torch.full((18, 10, 128), 7.0, device="cuda").to(BF)
-    lse = torch.full((18, 8), 7.0, device="cuda")
+    buf = torch.full((N + 4, 10, 128), 7.0, device="cuda").to(BF)
+    lse = torch.full((N + 4, 8), 7.0, device="cuda")
     paged.paged_attention(d["q"], d["k_cache"], d["v_cache"], d["block_table"], d["kv_lens"], d["q_starts"],
                           scale=0.2, out=buf[:, 2:], lse=lse)
     compare(d, buf[:, 2:], lse, scale=0.2)
     assert bool((buf[:, :2] == 7.0).all())
 
 
+@pytest.mark.parametrize("heads", [4, 32, 128])
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("tree", [False, True])
-def test_masked_places_may_hold_anything(bits, tree):
+def test_masked_places_may_hold_anything(bits, tree, heads):
     """NaN and infinities in rows past the keys, in unused pages and in new tokens that a row does not
     see leave that row's result as it was; rows that see them become NaN or infinite."""
     new, keys = [6, 3], [70, 35]
-    d = make_batch(new, keys, 4, 2, 128, 16, BF, bits, tree, seed=11)
+    d = make_batch(new, keys, heads, 2, 128, 16, BF, bits, tree, seed=11)
     if tree:
         sees = torch.tensor([[1, 3, 5, 9, 17, 33], [1, 3, 7, 0, 0, 0]], dtype=torch.int32, device="cuda")
         d["tree"] = torch.cat([sees[0], sees[1, :3]])[:, None].contiguous()
@@ -200,10 +211,11 @@ def test_masked_places_may_hold_anything(bits, tree):
                 assert torch.equal(out[i], good[i]), i
 
 
+@pytest.mark.parametrize("heads", [4, 48, 128])
 @pytest.mark.parametrize("bits", [16, 4])
-def test_bad_pages_are_left_out_and_reported(bits):
+def test_bad_pages_are_left_out_and_reported(bits, heads):
     from ae_b200 import paged
-    d = make_batch([2, 4], [200, 90], 4, 2, 64, 16, FP, bits, False, seed=2)
+    d = make_batch([2, 4], [200, 90], heads, 2, 64, 16, FP, bits, False, seed=2)
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     call(d, status=status)
     assert int(status) == 0
