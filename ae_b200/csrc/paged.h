@@ -51,6 +51,14 @@ struct Kv4ReadArgs {
   void* out;  // [M, Hkv, D]
 };
 
+// A segment whose keys were shared out over several CTAs, as its first CTA notes it.
+struct JoinRecord {
+  int last;         // last CTA with a part, -1: nothing to join
+  int slot;         // slot of the first part; CTA p's is 2 p
+  int head, heads;  // first query head, heads of a token
+  int tok, rows;    // first row of q, rows of the tile (tokens x gs)
+};
+
 struct AttnArgs {
   PagedCacheArgs c;
   const void* q;
@@ -72,7 +80,8 @@ struct AttnArgs {
   int* status;     // or null
   float* part_o;   // [2 * grid][R][D] unnormalised partial outputs
   float* part_ml;  // [2 * grid][R][2] their running maximum (log2 units) and sum
-  int min_tiles;   // fewest key tiles worth a CTA of its own
+  JoinRecord* records;  // [grid]
+  int min_tiles;        // fewest key tiles worth a CTA of its own
 };
 
 cudaError_t launch_kv_append(const AppendArgs& a, int D, bool bf16, bool bits4, int sms, cudaStream_t stream, bool pdl);
@@ -93,7 +102,6 @@ bool tc_takes(const PagedCacheArgs& c);
 bool plan_attn_tc(int N, int B, int g, int D, bool bits4, int sms, AttnPlan* p);
 cudaError_t launch_attn_tc(AttnArgs a, const AttnPlan& p, int D, bool bf16, cudaStream_t stream, bool pdl, bool* fits);
 // joins the partial results of the segments that were split over CTAs
-cudaError_t launch_attn_join(const AttnArgs& a, const AttnPlan& p, int key_tile, int D, bool bf16, cudaStream_t stream,
-                             bool pdl);
+cudaError_t launch_attn_join(const AttnArgs& a, const AttnPlan& p, int D, bool bf16, cudaStream_t stream, bool pdl);
 
 }  // namespace smb

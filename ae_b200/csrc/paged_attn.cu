@@ -102,10 +102,12 @@ __global__ void __launch_bounds__(128, (MmaCfg<D, MT, BITS4>::CTAS > 2 && MT == 
   pdl_launch_dependents();
   const long long W = plan_build<BK>(a, &s_plan);
   const int cta = blockIdx.x;
-  const int Gc = plan_ctas(a, W, gridDim.x);
-  if (W == 0 || cta >= Gc) return;
-  const long long w_lo = share_begin(W, Gc, cta), w_hi = share_begin(W, Gc, cta + 1);
-  if (w_lo >= w_hi) return;
+  const Shares shares(a, W, gridDim.x);
+  if (W == 0 || cta >= shares.ctas) {
+    if (tid == 0) a.records[cta].last = -1;
+    return;
+  }
+  const long long w_lo = shares.begin(cta), w_hi = shares.begin(cta + 1);
   Cursor cur = plan_locate<BK>(a, &s_plan, w_lo);
   long long w = w_lo;
 
@@ -571,37 +573,31 @@ __global__ void __launch_bounds__(128, (MmaCfg<D, MT, BITS4>::CTAS > 2 && MT == 
       }
     }
     w += t1 - t0;
-    if (w >= w_hi) break;
+    if (w >= w_hi) {
+      if (tid == 0) leave_record(a, cta, shares, cur, cur.start >= w_lo && t1 < cur.tiles, w_lo);
+      break;
+    }
     plan_next<BK>(a, cur);
     __syncthreads();  // the merge buffer is the next segment's ring
   }
 }
 
 // Joins the parts of the segments that were cut: CTA c takes the segment that begins in share c
-// and runs past its end, a warp one row of it, the parts in the order of their shares.
-template <int D, int BK, typename T>
-__global__ void __launch_bounds__(kPlanThreads) paged_join_kernel(const __grid_constant__ AttnArgs a, int R, int grid) {
+// and runs past its end (as its record says), a warp one row of it, the parts in the order of their
+// shares.
+template <int D, typename T>
+__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ AttnArgs a, int R) {
   constexpr int V = D / 32;  // floats per lane
   using H = Half2<T>;
-  __shared__ PlanShared s_plan;
   pdl_wait_prior_grids();
   pdl_launch_dependents();
-  const long long W = plan_build<BK>(a, &s_plan);
-  const int Gc = plan_ctas(a, W, grid);
   const int c = blockIdx.x;
-  if (W == 0 || c >= Gc) return;
-  const long long hi = share_begin(W, Gc, c + 1);
-  if (share_begin(W, Gc, c) >= hi) return;
-  const Cursor cur = plan_locate<BK>(a, &s_plan, hi - 1);
-  if (cur.start < share_begin(W, Gc, c) || cur.start + cur.tiles <= hi) return;
-  const int last = share_owner(W, Gc, cur.start + cur.tiles - 1);
-  const int kvh = cur.vh / a.nsub, sub = cur.vh % a.nsub;
-  const int heads = min(a.gs, a.g - sub * a.gs);
-  const int tok0 = cur.qt * a.tq, rows = min(a.tq, cur.s.n - tok0) * a.gs;
-  const int lane = threadIdx.x & 31;
-  const long long first = 2ll * c + (cur.start > share_begin(W, Gc, c) ? 1 : 0);
-  for (int r = blockIdx.y * (kPlanThreads / 32) + (threadIdx.x >> 5); r < rows; r += gridDim.y * (kPlanThreads / 32)) {
-    if (r % a.gs >= heads) continue;
+  const JoinRecord rec = a.records[c];
+  if (rec.last < 0) return;
+  const int last = rec.last, lane = threadIdx.x & 31;
+  const long long first = rec.slot;
+  for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < rec.rows; r += gridDim.y * 4) {
+    if (r % a.gs >= rec.heads) continue;
     float top = kNegInf;
     for (int p = c + lane; p <= last; p += 32)
       top = fmaxf(top, a.part_ml[((p == c ? first : 2ll * p) * R + r) * 2]);
@@ -625,8 +621,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_join_kernel(const __grid_c
       }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const long long tok = cur.s.s0 + tok0 + r / a.gs;
-    const int head = kvh * a.g + sub * a.gs + r % a.gs;
+    const long long tok = rec.tok + r / a.gs;
+    const int head = rec.head + r % a.gs;
     T* dst = static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + lane * V;
 #pragma unroll
     for (int e = 0; e < V; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = H::pack(acc[e] * inv, acc[e + 1] * inv);
@@ -692,35 +688,31 @@ cudaError_t launch_attn_mma(AttnArgs a, const AttnPlan& p, int D, bool bf16, boo
   void* params[] = {&a};
   err = cudaLaunchKernelExC(&cfg, v.fn, params);
   if (err != cudaSuccess) return err;
-  return launch_attn_join(a, p, bits4 ? 128 : 64, D, bf16, stream, pdl);
+  return launch_attn_join(a, p, D, bf16, stream, pdl);
 }
 
-cudaError_t launch_attn_join(const AttnArgs& a, const AttnPlan& p, int key_tile, int D, bool bf16, cudaStream_t stream,
-                             bool pdl) {
-  const void* fn = nullptr;
-#define SMB_JOIN(d, bk)                                                                              \
-  if (D == d && key_tile == bk)                                                                      \
-    fn = bf16 ? reinterpret_cast<const void*>(paged_join_kernel<d, bk, __nv_bfloat16>)               \
-              : reinterpret_cast<const void*>(paged_join_kernel<d, bk, __half>);
-  SMB_JOIN(64, 64)
-  SMB_JOIN(64, 128)
-  SMB_JOIN(128, 64)
-  SMB_JOIN(128, 128)
-  SMB_JOIN(256, 64)
-  SMB_JOIN(256, 128)
-#undef SMB_JOIN
-  if (fn == nullptr) return cudaErrorInvalidValue;
-  int R = p.rows, grid = p.grid;
+cudaError_t launch_attn_join(const AttnArgs& a, const AttnPlan& p, int D, bool bf16, cudaStream_t stream, bool pdl) {
+  const void* fn;
+  if (D == 64)
+    fn = bf16 ? reinterpret_cast<const void*>(paged_join_kernel<64, __nv_bfloat16>)
+              : reinterpret_cast<const void*>(paged_join_kernel<64, __half>);
+  else if (D == 128)
+    fn = bf16 ? reinterpret_cast<const void*>(paged_join_kernel<128, __nv_bfloat16>)
+              : reinterpret_cast<const void*>(paged_join_kernel<128, __half>);
+  else
+    fn = bf16 ? reinterpret_cast<const void*>(paged_join_kernel<256, __nv_bfloat16>)
+              : reinterpret_cast<const void*>(paged_join_kernel<256, __half>);
+  int R = p.rows;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.grid, (R + 15) / 16);
-  cfg.blockDim = dim3(kPlanThreads);
+  cfg.blockDim = dim3(128);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
-  void* params[] = {const_cast<AttnArgs*>(&a), &R, &grid};
+  void* params[] = {const_cast<AttnArgs*>(&a), &R};
   return cudaLaunchKernelExC(&cfg, fn, params);
 }
 

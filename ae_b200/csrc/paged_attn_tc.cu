@@ -25,8 +25,8 @@
 // a mask cuts a tile, the softmax warps look through V in shared memory before the product, take
 // non-finite values out, and the rows that do see them get them added from memory at the end.
 //
-// Every wait is bounded.  After a failed one all roles run on to the end of their loops without
-// waiting (their results are void, the status says so), so barriers between warps still match.
+// Every wait is bounded, and no role waits at a hardware barrier inside its loop: after a failed wait
+// each role runs out of segments by itself (the results are void, the status says so).
 #include <algorithm>
 #include <type_traits>
 
@@ -41,9 +41,8 @@ namespace {
 
 constexpr int kTBK = 128;       // keys of a tile
 constexpr int kTSlots = 5;      // ring slots
-constexpr int kTThreads = 384;  // warp 0 TMA, warp 1 MMA, warp 2 TMEM, warp 3 idle, warps 4-7 / 8-11 softmax
+constexpr int kTThreads = 384;  // warp 0 TMA, warp 1 MMA, warp 2 TMEM, warp 3 segments, warps 4-7 / 8-11 softmax
 constexpr int kTOkRing = 8;     // tiles whose page masks are kept: the ring lets K run at most 5 tiles ahead
-enum : int { kFixValues = 1, kFixBadPage = 2 };  // this CTA met non-finite values behind a mask / bad pages
 
 template <int D, bool DUAL>
 struct TcCfg {
@@ -106,34 +105,62 @@ __device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t (&v)[32
 __device__ __forceinline__ void tmem_ld_done(uint32_t (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : SMB_P16(v, 0), SMB_P16(v, 16) : : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+// The same for 16 columns.
+__device__ __forceinline__ void tmem_ld16_wait(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      SMB_I16(v, 0), SMB_I16(v, 16)
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];\n\ttcgen05.wait::ld.sync.aligned;"
+      : SMB_R16(v, 0)
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      SMB_I16(v, 0)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void named_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
-// The segments of this CTA's share, walked alike by every role.
-struct Walk {
-  Cursor cur;
-  long long w, w_hi;
-  int t0, t1;
-  __device__ __forceinline__ void open() {
-    t0 = cur.tile;
-    t1 = static_cast<int>(min(static_cast<long long>(cur.tiles), cur.tile + (w_hi - w)));
-  }
-  __device__ __forceinline__ bool next(const AttnArgs& a) {
-    w += t1 - t0;
-    if (w >= w_hi) return false;
-    plan_next<kTBK>(a, cur);
-    open();
-    return true;
-  }
+// Two 32-bit values in one instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// One segment of this CTA's share.  Warp 3 walks the share and hands them to the other roles.
+struct Segment {
+  int t0, t1;         // its key tiles (t1 = -1: the share is done)
+  int keys;           // keys its rows can see
+  int prefix, open;   // keys before the new tokens; first key that some row may not see
+  int b, kvh;
+  int head, heads;    // first query head, heads of a token
+  int tok, toks, i0;  // first row of q, tokens, the first one's place among the sequence's new tokens
+  int slot;           // of a partial result, -1: the segment lies in this share
 };
+constexpr int kTSegs = 4;                  // segments handed out ahead
+constexpr int kTSegReaders = 1 + 1 + 256;  // TMA and MMA warps, softmax threads
 
 template <int D, bool DUAL, typename T>
 __global__ void __launch_bounds__(kTThreads, 1)
@@ -146,7 +173,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
   constexpr uint32_t HALF = kTBK * 128;  // bytes of 64 dims of a tile
   extern __shared__ uint8_t dyn_smem[];
   __shared__ PlanShared s_plan;
-  __shared__ uint64_t full_bar[kTSlots], empty_bar[kTSlots], s_bar[2], p_bar[2], o_bar[2], q_bar[2], drain_bar;
+  __shared__ uint64_t full_bar[kTSlots], empty_bar[kTSlots], s_bar[2], p_bar[2][2], o_bar[2], q_bar[2], drain_bar, both_bar;
+  __shared__ uint64_t seg_full[kTSegs], seg_empty[kTSegs];
+  __shared__ Segment s_seg[kTSegs];
   __shared__ uint32_t s_tmem, s_pages[kTOkRing];
   __shared__ int s_abort, s_fix;
   __shared__ float2 s_ml[DUAL ? 1 : 128];
@@ -166,11 +195,17 @@ __global__ void __launch_bounds__(kTThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_bar[i], 1);
-      mbar_init(&p_bar[i], 128);
+      mbar_init(&p_bar[i][0], 128);
+      mbar_init(&p_bar[i][1], 128);
       mbar_init(&o_bar[i], 1);
       mbar_init(&q_bar[i], 128);
     }
+    for (int i = 0; i < kTSegs; ++i) {
+      mbar_init(&seg_full[i], 1);
+      mbar_init(&seg_empty[i], kTSegReaders);
+    }
     mbar_init(&drain_bar, 1);
+    mbar_init(&both_bar, 256);
     fence_mbarrier_init();
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
@@ -187,20 +222,23 @@ __global__ void __launch_bounds__(kTThreads, 1)
   pdl_wait_prior_grids();
   pdl_launch_dependents();
   const long long W = plan_build<kTBK>(a, &s_plan);
-  const int Gc = plan_ctas(a, W, gridDim.x);
+  const Shares shares(a, W, gridDim.x);
   const int cta = blockIdx.x;
-  const long long w_lo = W > 0 && cta < Gc ? share_begin(W, Gc, cta) : 0;
-  const long long w_hi = W > 0 && cta < Gc ? share_begin(W, Gc, cta + 1) : 0;
+  const bool works = W > 0 && cta < shares.ctas;
+  const long long w_lo = works ? shares.begin(cta) : 0, w_hi = works ? shares.begin(cta + 1) : 0;
+  if (!works && tid == 0) a.records[cta].last = -1;
   int* status = a.status;
   volatile int* abort_flag = &s_abort;
 
-  if (w_lo < w_hi) {
-    Walk k;
-    k.cur = plan_locate<kTBK>(a, &s_plan, w_lo);
-    k.w = w_lo;
-    k.w_hi = w_hi;
-    k.open();
-
+  if (works) {
+    // The i-th segment of the share; false when it is done, or after a failed wait.
+    auto next_segment = [&](int i, Segment& g) {
+      if (!mbar_wait(&seg_full[i % kTSegs], (i / kTSegs) & 1, status, abort_flag)) return false;
+      g = s_seg[i % kTSegs];
+      return g.t1 >= 0;
+    };
+    Segment g{};
+    int seg = 0;
     if (warp < 4) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
       if (warp == 0) {
@@ -213,17 +251,14 @@ __global__ void __launch_bounds__(kTThreads, 1)
         auto load = [&](const CUtensorMap* map, int t, bool is_k) {
           const int slot = it % kTSlots;
           const int p = lane % pages, j = t * kTBK + p * psb;
-          const bool in = j < k.cur.keys;
-          const int page = in ? a.table[k.cur.b * a.table_stride + (j >> a.c.page_shift)] : -1;
+          const bool in = j < g.keys;
+          const int page = in ? a.table[g.b * a.table_stride + (j >> a.c.page_shift)] : -1;
           const bool good = page >= 0 && page < a.c.num_pages;
           const uint32_t bad = __ballot_sync(0xffffffffu, in && lane < pages && !good);
           if (is_k) {
             if (lane == 0) {
               s_pages[tc % kTOkRing] = ~bad;
-              if (bad != 0) {
-                record_status(status, kDevBadPage);
-                atomicOr(&s_fix, kFixBadPage);
-              }
+              if (bad != 0) record_status(status, kDevBadPage);
             }
             ++tc;
           }
@@ -233,34 +268,67 @@ __global__ void __launch_bounds__(kTThreads, 1)
           if (lane < boxes) {
             const int h = lane / pages;
             tma_load_4d(ring_s + slot * TILE + h * HALF + p * psb * 128, map, &full_bar[slot], h * 64, j & page_mask,
-                        k.cur.vh / a.nsub, good ? page : static_cast<int>(a.c.num_pages));
+                        g.kvh, good ? page : static_cast<int>(a.c.num_pages));
           }
           ++it;
         };
-        do {
-          const int n = k.t1 - k.t0;
+        while (__all_sync(0xffffffffu, next_segment(seg, g))) {
+          if (lane == 0) mbar_arrive(&seg_empty[seg % kTSegs]);
+          ++seg;
+          const int n = g.t1 - g.t0;
           if constexpr (DUAL) {
-            for (int t = k.t0; t < k.t1; ++t) {
+            for (int t = g.t0; t < g.t1; ++t) {
               load(&tm_k, t, true);
               load(&tm_v, t, false);
             }
           } else {
-            load(&tm_k, k.t0, true);
-            if (n > 1) load(&tm_k, k.t0 + 1, true);
+            load(&tm_k, g.t0, true);
+            if (n > 1) load(&tm_k, g.t0 + 1, true);
             for (int i = 0; i < n; ++i) {
-              load(&tm_v, k.t0 + i, false);
-              if (i + 2 < n) load(&tm_k, k.t0 + i + 2, true);
+              load(&tm_v, g.t0 + i, false);
+              if (i + 2 < n) load(&tm_k, g.t0 + i + 2, true);
             }
           }
-        } while (k.next(a));
+        }
         // the copies into every slot have landed before the CTA may end
         for (int i = max(0, it - kTSlots); i < it; ++i)
           mbar_wait(&full_bar[i % kTSlots], (i / kTSlots) & 1, status, nullptr);
+      } else if (warp == 3 && lane == 0) {
+        // ---------------------------------------------------------------- segments
+        Cursor cur = plan_locate<kTBK>(a, &s_plan, w_lo);
+        for (long long w = w_lo; w < w_hi; ++seg) {
+          Segment n;
+          n.t0 = cur.tile;
+          n.t1 = static_cast<int>(min(static_cast<long long>(cur.tiles), cur.tile + (w_hi - w)));
+          n.keys = cur.keys;
+          const int sub = cur.vh % a.nsub;
+          n.kvh = cur.vh / a.nsub;
+          n.b = cur.b;
+          n.head = n.kvh * a.g + sub * a.gs;
+          n.heads = min(a.gs, a.g - sub * a.gs);
+          n.i0 = cur.qt * a.tq;
+          n.tok = cur.s.s0 + n.i0;
+          n.toks = min(a.tq, cur.s.n - n.i0);
+          n.prefix = cur.s.L - cur.s.n;
+          n.open = a.tree != nullptr ? n.prefix : n.prefix + n.i0 + 1;
+          n.slot = n.t0 == 0 && n.t1 == cur.tiles ? -1 : 2 * cta + (cur.start > w_lo ? 1 : 0);
+          mbar_wait(&seg_empty[seg % kTSegs], ((seg / kTSegs) & 1) ^ 1, status, abort_flag);
+          s_seg[seg % kTSegs] = n;
+          mbar_arrive(&seg_full[seg % kTSegs]);
+          w += n.t1 - n.t0;
+          if (w >= w_hi)
+            leave_record(a, cta, shares, cur, cur.start >= w_lo && n.t1 < cur.tiles, w_lo);
+          else
+            plan_next<kTBK>(a, cur);
+        }
+        mbar_wait(&seg_empty[seg % kTSegs], ((seg / kTSegs) & 1) ^ 1, status, abort_flag);
+        s_seg[seg % kTSegs].t1 = -1;
+        mbar_arrive(&seg_full[seg % kTSegs]);
       } else if (warp == 1 && lane == 0) {
         // ---------------------------------------------------------------- MMA
         constexpr uint32_t idesc_s = idesc_f16(kBF16, 128, kTBK);
         constexpr uint32_t idesc_o = idesc_f16(kBF16, 128, D) | kIdescBMn;
-        int it = 0, np[2] = {0, 0}, seg = 0;
+        int it = 0, np[2] = {0, 0};
         auto wait_full = [&](int i) {
           mbar_wait(&full_bar[i % kTSlots], (i / kTSlots) & 1, status, abort_flag);
           tc_fence_after();
@@ -273,20 +341,23 @@ __global__ void __launch_bounds__(kTThreads, 1)
             umma_f16(tmem + kTmemS + s * 128, desc_kmajor_sw128(qs + off), desc_kmajor_sw128(ks + off), idesc_s, kk > 0);
           }
         };
-        auto pv = [&](int i, int s, bool first) {  // O_s (+)= P_s V
+        // O_s (+)= P_s V, each half as soon as its 64 keys of P are there
+        auto pv = [&](int i, int s, bool first) {
           const uint32_t vs = ring_s + (i % kTSlots) * TILE;
 #pragma unroll
-          for (int kk = 0; kk < kTBK / 16; ++kk)
-            umma_f16_ts(tmem + kTmemO + s * 128, tmem + kTmemS + s * 128 + kk * 8,
-                        desc_mnmajor_sw128(vs + kk * 2048, HALF), idesc_o, !(first && kk == 0));
-        };
-        auto wait_p = [&](int s) {
-          mbar_wait(&p_bar[s], np[s] & 1, status, abort_flag);
+          for (int h = 0; h < 2; ++h) {
+            mbar_wait(&p_bar[s][h], np[s] & 1, status, abort_flag);
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+              umma_f16_ts(tmem + kTmemO + s * 128, tmem + kTmemS + s * 128 + kk * 8,
+                          desc_mnmajor_sw128(vs + kk * 2048, HALF), idesc_o, !(first && kk == 0));
+          }
           ++np[s];
-          tc_fence_after();
         };
-        do {
-          const int n = k.t1 - k.t0;
+        while (next_segment(seg, g)) {
+          mbar_arrive(&seg_empty[seg % kTSegs]);
+          const int n = g.t1 - g.t0;
           mbar_wait(&q_bar[0], seg & 1, status, abort_flag);
           mbar_wait(&q_bar[1], seg & 1, status, abort_flag);
           tc_fence_after();
@@ -304,7 +375,6 @@ __global__ void __launch_bounds__(kTThreads, 1)
               const int vslot = it++;
               if (more) kslot = it++;
               wait_full(vslot);
-              wait_p(0);
               pv(vslot, 0, t == 0);
               if (more) {
                 wait_full(kslot);
@@ -313,7 +383,6 @@ __global__ void __launch_bounds__(kTThreads, 1)
               } else {
                 umma_commit(&o_bar[0]);
               }
-              wait_p(1);
               pv(vslot, 1, t == 0);
               umma_commit(&empty_bar[vslot % kTSlots]);
               if (more) {
@@ -335,7 +404,6 @@ __global__ void __launch_bounds__(kTThreads, 1)
             for (int t = 0; t < n; ++t) {
               const int s = t & 1;
               wait_full(it);
-              wait_p(s);
               pv(it, s, t < 2);
               umma_commit(&empty_bar[it % kTSlots]);
               ++it;
@@ -350,7 +418,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
               }
             }
           }
-        } while (k.next(a));
+        }
         umma_commit(&drain_bar);
         mbar_wait(&drain_bar, 0, status, nullptr);
       }
@@ -364,24 +432,28 @@ __global__ void __launch_bounds__(kTThreads, 1)
       const uint32_t t_s = t_lane + kTmemS + s * 128, t_o = t_lane + kTmemO + s * 128;
       int it = 0, tc = 0, ns = 0, no = 0;
       const int tok_r = r / a.gs, sub_r = r % a.gs;
-      do {
-        const int n = k.t1 - k.t0;
-        const Cursor& cur = k.cur;
-        const int kvh = cur.vh / a.nsub, sub = cur.vh % a.nsub;
-        const int heads = min(a.gs, a.g - sub * a.gs);
-        const int tok0 = cur.qt * a.tq, toks = min(a.tq, cur.s.n - tok0);
-        const int prefix = cur.s.L - cur.s.n;
-        const bool row_ok = tok_r < toks && sub_r < heads;
-        const int open = a.tree != nullptr ? prefix : prefix + tok0 + 1;  // first key some row may not see
-        const long long tok = cur.s.s0 + tok0 + tok_r;
-        const int head = kvh * a.g + sub * a.gs + sub_r;
+      int nb = 0;
+      auto both = [&]() {  // the streams meet (bounded, unlike a named barrier)
+        __syncwarp();
+        mbar_arrive(&both_bar);
+        mbar_wait(&both_bar, nb & 1, status, abort_flag);
+        __syncwarp();
+        ++nb;
+      };
+      while (__all_sync(0xffffffffu, next_segment(seg, g))) {
+        mbar_arrive(&seg_empty[seg % kTSegs]);
+        ++seg;
+        const int n = g.t1 - g.t0;
+        const bool row_ok = tok_r < g.toks && sub_r < g.heads;
+        const long long tok = g.tok + tok_r;
+        const int head = g.head + sub_r;
         // ---- Q: 16-byte chunks of a row, swizzled as TMA would write them
         {
           const int rq = DUAL ? r : (tid - 128) & 127;
           const int tokq = rq / a.gs, subq = rq % a.gs;
-          const bool okq = tokq < toks && subq < heads;
-          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (cur.s.s0 + tok0 + tokq) * a.q_ts +
-                                                            (kvh * a.g + sub * a.gs + subq) * a.q_hs);
+          const bool okq = tokq < g.toks && subq < g.heads;
+          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (g.tok + tokq) * a.q_ts +
+                                                            (g.head + subq) * a.q_hs);
           constexpr int CH = D / 8;
           const int c0 = DUAL ? 0 : s * (CH / 2), c1 = DUAL ? CH : c0 + CH / 2;
           const int rr = rq & 127;
@@ -397,19 +469,47 @@ __global__ void __launch_bounds__(kTThreads, 1)
         }
         float m = kNegInf, l = 0.f;
         auto visible = [&](int j) {  // this row, key j
-          if (!row_ok || j >= cur.keys) return false;
-          const int lj = j - prefix;
-          if (a.tree == nullptr) return lj <= tok0 + tok_r;
+          if (!row_ok || j >= g.keys) return false;
+          const int lj = j - g.prefix;
+          if (a.tree == nullptr) return lj <= g.i0 + tok_r;
           if (lj < 0) return true;
           return (lj >> 5) < a.tree_words &&
                  ((static_cast<uint32_t>(a.tree[tok * a.tree_stride + (lj >> 5)]) >> (lj & 31)) & 1u) != 0;
         };
         for (int i = DUAL ? 0 : s; i < n; i += DUAL ? 1 : 2) {
-          const int j0 = (k.t0 + i) * kTBK;
+          const int j0 = (g.t0 + i) * kTBK;
+          const bool cut = j0 + kTBK > g.open || j0 + kTBK > g.keys;
+          if (cut) {
+            // V: what no mask stops from entering the product has to be finite
+            const int vstep = it + (DUAL ? 2 * i + 1 : i + min(i + 2, n));
+            mbar_wait(&full_bar[vstep % kTSlots], (vstep / kTSlots) & 1, status, abort_flag);
+            uint8_t* vp = sm + C::Q + (vstep % kTSlots) * TILE + row * 128;
+            const bool dead = j0 + row >= g.keys;  // a row behind the keys
+            bool bad = false;
+#pragma unroll 4
+            for (int c = 0; c < D / 8; ++c) {
+              uint4* p = reinterpret_cast<uint4*>(vp + (c >> 3) * HALF + ((c & 7) << 4));
+              uint4 v = *p;
+              uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+              bool hit = false;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (H::nonfinite(u[e] & 0xffffu)) u[e] &= 0xffff0000u, hit = true;
+                if (H::nonfinite(u[e] >> 16)) u[e] &= 0xffffu, hit = true;
+              }
+              if (hit) {
+                bad = true;
+                if (!dead) *reinterpret_cast<volatile int*>(&s_fix) = 1;  // before the value goes
+                __threadfence_block();
+                *p = v;
+              }
+            }
+            if (bad) fence_async_proxy();
+          }
           mbar_wait(&s_bar[s], ns & 1, status, abort_flag);
           tc_fence_after();
           const uint32_t pages_ok = s_pages[(tc + i) % kTOkRing];
-          const bool masked = j0 + kTBK > open || j0 + kTBK > cur.keys || pages_ok != 0xffffffffu;
+          const bool masked = cut || pages_ok != 0xffffffffu;
           uint32_t x[4][32];
 #pragma unroll
           for (int q = 0; q < 4; ++q) tmem_ld32_issue(t_s + q * 32, x[q]);
@@ -421,12 +521,12 @@ __global__ void __launch_bounds__(kTThreads, 1)
             for (int q = 0; q < 4; ++q) {
               const int jq = j0 + q * 32;
               uint32_t see = 0;  // bit e: this row sees key jq + e
-              const int left = min(32, cur.keys - jq);
+              const int left = min(32, g.keys - jq);
               if (row_ok && left > 0) {
                 see = left == 32 ? 0xffffffffu : (1u << left) - 1u;
-                const int lj = jq - prefix;
+                const int lj = jq - g.prefix;
                 if (a.tree == nullptr) {
-                  const int c = tok0 + tok_r - lj + 1;
+                  const int c = g.i0 + tok_r - lj + 1;
                   see &= c >= 32 ? 0xffffffffu : c <= 0 ? 0u : (1u << c) - 1u;
                 } else if (lj > -32) {
                   const int w0 = lj >> 5, sh = lj & 31;  // (floor: lj may be negative)
@@ -444,38 +544,14 @@ __global__ void __launch_bounds__(kTThreads, 1)
               for (int e = 0; e < 32; ++e)
                 if (!((see >> e) & 1u)) x[q][e] = __float_as_uint(kNegInf);
             }
-            // V: what no mask stops from entering the product has to be finite
-            const int vstep = it + (DUAL ? 2 * i + 1 : i + min(i + 2, n));
-            mbar_wait(&full_bar[vstep % kTSlots], (vstep / kTSlots) & 1, status, abort_flag);
-            uint8_t* vp = sm + C::Q + (vstep % kTSlots) * TILE + row * 128;
-            const bool dead = j0 + row >= cur.keys;  // a row behind the keys
-            bool bad = false;
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-              uint4* p = reinterpret_cast<uint4*>(vp + (c >> 3) * HALF + ((c & 7) << 4));
-              uint4 v = *p;
-              uint32_t* u = reinterpret_cast<uint32_t*>(&v);
-              bool hit = false;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if (H::nonfinite(u[e] & 0xffffu)) u[e] &= 0xffff0000u, hit = true;
-                if (H::nonfinite(u[e] >> 16)) u[e] &= 0xffffu, hit = true;
-              }
-              if (hit) {
-                bad = true;
-                if (!dead) atomicOr(&s_fix, kFixValues);  // before the value goes
-                __threadfence_block();
-                *p = v;
-              }
-            }
-            if (bad) fence_async_proxy();
           }
 
           float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
 #pragma unroll
           for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(x[q][e]));
+            for (int e = 0; e < 32; e += 2)
+              top[(e >> 1) & 3] = max3(top[(e >> 1) & 3], __uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1]));
           const float tmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
           // a row is rescaled only when its maximum grew by more than 8 (p stays below 2^8)
           const bool grew = tmax > m + 8.f;
@@ -486,37 +562,42 @@ __global__ void __launch_bounds__(kTThreads, 1)
             l *= f;
             if (i >= (DUAL ? 1 : 2)) {
               // (this stream's last product is complete: it was issued before the S just waited for)
+#pragma unroll 2
+              for (int q = 0; q < D / 16; ++q) {
+                uint32_t o[16];
+                tmem_ld16_wait(t_o + q * 16, o);
 #pragma unroll
-              for (int q = 0; q < D / 32; ++q) {
-                uint32_t o[32];
-                tmem_ld32_issue(t_o + q * 32, o);
-                tmem_ld_done(o);
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tmem_st32(t_o + q * 32, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st16(t_o + q * 16, o);
               }
               tmem_st_done();
             }
           }
           const float mm = m == kNegInf ? 0.f : m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), mm2 = pair(-mm, -mm);
+          uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            uint32_t p[32];
+          for (int q = 0; q < 4; ++q) {
+            uint32_t p[16];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float v0 = exp2_fast(fmaf(__uint_as_float(x[2 * q + e / 16][(e % 16) * 2]), a.scale_log2, -mm));
-              const float v1 = exp2_fast(fmaf(__uint_as_float(x[2 * q + e / 16][(e % 16) * 2 + 1]), a.scale_log2, -mm));
-              sum[e & 1] += v0;
-              sum[2 + (e & 1)] += v1;
+            for (int e = 0; e < 16; ++e) {
+              float v0, v1;
+              unpair(fma2(pair(__uint_as_float(x[q][2 * e]), __uint_as_float(x[q][2 * e + 1])), scale2, mm2), v0, v1);
+              v0 = exp2_fast(v0);
+              v1 = exp2_fast(v1);
+              sum[e & 1] = add2(sum[e & 1], pair(v0, v1));
               p[e] = H::pack(v0, v1);
             }
-            tmem_st32(t_s + q * 32, p);
+            tmem_st16(t_s + q * 16, p);
+            if (q & 1) {  // the product starts on the first 64 keys while the others are worked on
+              tmem_st_done();
+              tc_fence_before();
+              mbar_arrive(&p_bar[s][q >> 1]);
+            }
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tmem_st_done();
-          tc_fence_before();
-          mbar_arrive(&p_bar[s]);
+          float s0, s1;
+          unpair(add2(sum[0], sum[1]), s0, s1);
+          l += s0 + s1;
           ++ns;
         }
 
@@ -527,22 +608,22 @@ __global__ void __launch_bounds__(kTThreads, 1)
           ++no;
           tc_fence_after();
         }
-        const bool whole = k.t0 == 0 && k.t1 == cur.tiles;
-        const long long slot = 2ll * cta + (cur.start > w_lo ? 1 : 0);
+        const bool whole = g.slot < 0;
+        const long long slot = g.slot;
         float f0 = 1.f, f1 = 0.f;
         if constexpr (!DUAL) {
           if (s == 1) s_ml[row] = make_float2(m, l);
-          named_sync(1, 256);
+          both();
           if (s == 0) {
             const float2 o = s_ml[row];
-            const float both = fmaxf(m, o.x);
-            f0 = m == kNegInf ? 1.f : exp2_fast(m - both);
-            f1 = o.x == kNegInf ? 1.f : exp2_fast(o.x - both);
+            const float mx = fmaxf(m, o.x);
+            f0 = m == kNegInf ? 1.f : exp2_fast(m - mx);
+            f1 = o.x == kNegInf ? 1.f : exp2_fast(o.x - mx);
             l = l * f0 + o.y * f1;
-            m = both;
+            m = mx;
           }
         }
-        const int fix = *reinterpret_cast<volatile int*>(&s_fix);
+        const bool fix = *reinterpret_cast<volatile int*>(&s_fix) != 0;
         float inv = 1.f;
         if (whole) inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -556,16 +637,16 @@ __global__ void __launch_bounds__(kTThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0u;
           }
-          if ((fix & kFixValues) && row_ok) {
+          if (fix && row_ok) {
             // non-finite values that were taken out of this stream's masked tiles, and that this row sees
             for (int i = DUAL ? 0 : s; i < n; i += DUAL ? 1 : 2) {
-              const int j0 = (k.t0 + i) * kTBK;
-              if (j0 + kTBK <= open && j0 + kTBK <= cur.keys && !(fix & kFixBadPage)) continue;
-              for (int j = j0; j < min(j0 + kTBK, cur.keys); ++j) {
+              const int j0 = (g.t0 + i) * kTBK;
+              if (j0 + kTBK <= g.open && j0 + kTBK <= g.keys) continue;
+              for (int j = j0; j < min(j0 + kTBK, g.keys); ++j) {
                 if (!visible(j)) continue;
-                const int page = a.table[cur.b * a.table_stride + (j >> a.c.page_shift)];
+                const int page = a.table[g.b * a.table_stride + (j >> a.c.page_shift)];
                 if (page < 0 || page >= a.c.num_pages) continue;
-                const T* v = reinterpret_cast<const T*>(a.c.v + page * a.c.page_stride + kvh * a.c.head_stride +
+                const T* v = reinterpret_cast<const T*>(a.c.v + page * a.c.page_stride + g.kvh * a.c.head_stride +
                                                         (j & ((1 << a.c.page_shift) - 1)) * a.c.token_stride) + q * 32;
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
@@ -582,13 +663,13 @@ __global__ void __launch_bounds__(kTThreads, 1)
               for (int e = 0; e < 32; ++e) merge[e * 128 + row] = __uint_as_float(o[e]);
             }
             __syncwarp();
-            named_sync(1, 256);
+            both();
             if (s == 0) {
 #pragma unroll
               for (int e = 0; e < 32; ++e)
                 o[e] = __float_as_uint(__uint_as_float(o[e]) * f0 + merge[e * 128 + row] * f1);
             }
-            named_sync(1, 256);  // the next columns go to the same place
+            both();  // the next columns go to the same place
           }
           if ((DUAL || s == 0) && row_ok) {
             if (whole) {
@@ -620,8 +701,8 @@ __global__ void __launch_bounds__(kTThreads, 1)
         it += 2 * n;
         tc += n;
         __syncwarp();
-        if constexpr (!DUAL) named_sync(1, 256);  // both streams are done with Q and (m, l)
-      } while (k.next(a));
+        if constexpr (!DUAL) both();  // both streams are done with Q and (m, l)
+      }
     }
   }
   __syncwarp();
@@ -697,7 +778,7 @@ cudaError_t launch_attn_tc(AttnArgs a, const AttnPlan& p, int D, bool bf16, cuda
   void* params[] = {&a, &tk, &tv};
   err = cudaLaunchKernelExC(&cfg, fn, params);
   if (err != cudaSuccess) return err;
-  return launch_attn_join(a, p, kTBK, D, bf16, stream, pdl);
+  return launch_attn_join(a, p, D, bf16, stream, pdl);
 }
 
 }  // namespace smb

@@ -51,7 +51,7 @@ int attn_sizes(int N, int B, int Hq, int Hkv, int D, int bits) {
 }
 
 size_t attn_ws(const AttnPlan& p, int D) {
-  return static_cast<size_t>(2) * p.grid * p.rows * (D + 2) * sizeof(float);
+  return static_cast<size_t>(2) * p.grid * p.rows * (D + 2) * sizeof(float) + p.grid * sizeof(JoinRecord);
 }
 
 }  // namespace
@@ -214,6 +214,7 @@ int smb_paged_attention(const smb_paged_cache_t* cache, const void* q, int64_t q
     a.tq = p.rows / a.gs;
     a.part_o = static_cast<float*>(ws);
     a.part_ml = a.part_o + static_cast<size_t>(2) * p.grid * p.rows * D;
+    a.records = reinterpret_cast<JoinRecord*>(a.part_ml + static_cast<size_t>(4) * p.grid * p.rows);
     a.min_tiles = 2;
     return ws_bytes >= attn_ws(p, D);
   };

@@ -8,7 +8,8 @@
 // that lies inside one share is finished by its CTA; one that is cut leaves a partial result in
 // at most two slots per CTA (2c: the segment its share begins in, 2c + 1: the one it ends in),
 // and a second kernel joins the parts in the order of their CTAs, so the result does not depend
-// on timing.  The slots' size follows the grid and not the lengths.
+// on timing.  The slots' size follows the grid and not the lengths.  The CTA in whose share a cut
+// segment begins leaves a record of it, so the second kernel plans nothing.
 #pragma once
 
 #include "common.cuh"
@@ -33,7 +34,9 @@ __device__ __forceinline__ Seq seq_at(const AttnArgs& a, int b) {
   return s;
 }
 
-__device__ __forceinline__ int row_tiles(const AttnArgs& a, const Seq& s) { return (s.n + a.tq - 1) / a.tq; }
+__device__ __forceinline__ int row_tiles(const AttnArgs& a, const Seq& s) {
+  return s.n <= a.tq ? (s.n > 0) : (s.n + a.tq - 1) / a.tq;
+}
 
 // Keys that row tile qt can see (all of them for a tree, up to its last token otherwise).
 __device__ __forceinline__ int keys_of_tile(const AttnArgs& a, const Seq& s, int qt) {
@@ -45,6 +48,12 @@ __device__ __forceinline__ int keys_of_tile(const AttnArgs& a, const Seq& s, int
 template <int BK>
 __device__ __forceinline__ int tiles_of(int keys) {
   return max(1, keys / BK + (keys % BK != 0));
+}
+
+// a / b, in 32 bits where both fit (a 64-bit division takes some 100 instructions).
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
 }
 
 // sum over i < n of floor((step * i + b) / BK), b >= 0
@@ -70,6 +79,7 @@ __device__ __forceinline__ long long floor_sum(long long n, long long step, long
 template <int BK>
 __device__ __forceinline__ long long tiles_before(const AttnArgs& a, const Seq& s, int qt) {
   if (qt <= 0) return 0;
+  if (s.n <= a.tq) return tiles_of<BK>(keys_of_tile(a, s, 0));
   if (a.tree != nullptr) return static_cast<long long>(qt) * tiles_of<BK>(s.L);
   const int all = row_tiles(a, s);
   long long sum = 0;
@@ -149,16 +159,17 @@ __device__ Cursor plan_locate(const AttnArgs& a, const PlanShared* sh, long long
   long long at = sh->before[lo];
   Cursor c;
   c.b = lo * per;
-  while (true) {  // w < W, so a sequence that holds it comes before B
-    c.s = seq_at(a, c.b);
+  c.s = seq_at(a, c.b);
+  for (int i = 1; i < per && c.b + 1 < a.B; ++i) {  // w < W, so a sequence that holds it comes before B
     const long long here = seq_tiles<BK>(a, c.s);
-    if (w < at + here || c.b + 1 >= a.B) break;
+    if (w < at + here) break;
     at += here;
     ++c.b;
+    c.s = seq_at(a, c.b);
   }
   const int qts = row_tiles(a, c.s);
   const long long per_head = max(1ll, tiles_before<BK>(a, c.s, qts));
-  c.vh = static_cast<int>((w - at) / per_head);
+  c.vh = static_cast<int>(quotient(w - at, per_head));
   at += c.vh * per_head;
   int l = 0, h = qts;
   while (h - l > 1) {
@@ -193,14 +204,39 @@ __device__ __forceinline__ void plan_next(const AttnArgs& a, Cursor& c) {
   c.tiles = tiles_of<BK>(c.keys);
 }
 
-// CTAs that get work: no share below min_tiles while that leaves CTAs idle.
-__device__ __forceinline__ int plan_ctas(const AttnArgs& a, long long W, int grid) {
-  const long long most = (W + a.min_tiles - 1) / a.min_tiles;
-  return static_cast<int>(min(static_cast<long long>(grid), max(1ll, most)));
-}
-__device__ __forceinline__ long long share_begin(long long W, int G, int c) { return W * c / G; }
-__device__ __forceinline__ int share_owner(long long W, int G, long long w) {
-  return static_cast<int>(((w + 1) * G - 1) / W);
+// The shares: CTA c of `ctas` takes [begin(c), begin(c + 1)), the first `more` one tile more than the
+// others.  No share is below min_tiles while that leaves CTAs idle.
+struct Shares {
+  long long each;
+  int more, ctas;
+  __device__ __forceinline__ Shares(const AttnArgs& a, long long W, int grid) {
+    ctas = static_cast<int>(min(static_cast<long long>(grid), max(1ll, quotient(W + a.min_tiles - 1, a.min_tiles))));
+    each = quotient(W, ctas);
+    more = static_cast<int>(W - each * ctas);
+  }
+  __device__ __forceinline__ long long begin(int c) const { return c * each + min(c, more); }
+  __device__ __forceinline__ int owner(long long w) const {
+    const long long head = more * (each + 1);
+    return static_cast<int>(w < head ? quotient(w, each + 1) : more + quotient(w - head, each));
+  }
+};
+
+// Notes for the join, by the CTA whose share ends with (c, t1): `first` = it is the segment's first
+// part and others follow.  Called by one thread, once.
+__device__ __forceinline__ void leave_record(const AttnArgs& a, int cta, const Shares& sh, const Cursor& c, bool cut,
+                                             long long w_lo) {
+  JoinRecord r;
+  r.last = -1;
+  if (cut) {
+    r.last = sh.owner(c.start + c.tiles - 1);
+    r.slot = 2 * cta + (c.start > w_lo ? 1 : 0);
+    const int kvh = c.vh / a.nsub, sub = c.vh % a.nsub;
+    r.heads = min(a.gs, a.g - sub * a.gs);
+    r.head = kvh * a.g + sub * a.gs;
+    r.rows = min(a.tq, c.s.n - c.qt * a.tq) * a.gs;
+    r.tok = c.s.s0 + c.qt * a.tq;
+  }
+  a.records[cta] = r;
 }
 
 }  // namespace smb
