@@ -78,7 +78,7 @@ struct AttnArgs {
   long long o_ts, o_hs;
   float* lse;      // [N, Hq] or null
   int* status;     // or null
-  float* part_o;   // [2 * grid][R][D] unnormalised partial outputs
+  float* part_o;   // [2 * grid][D][R] unnormalised partial outputs (rows innermost)
   float* part_ml;  // [2 * grid][R][2] their running maximum (log2 units) and sum
   JoinRecord* records;  // [grid]
   int min_tiles;        // fewest key tiles worth a CTA of its own

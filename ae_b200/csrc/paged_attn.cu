@@ -100,20 +100,17 @@ __global__ void __launch_bounds__(128, (MmaCfg<D, MT, BITS4>::CTAS > 2 && MT == 
 
   pdl_wait_prior_grids();
   pdl_launch_dependents();
-  const long long W = plan_build<BK>(a, &s_plan);
   const int cta = blockIdx.x;
-  const Shares shares(a, W, gridDim.x);
-  if (W == 0 || cta >= shares.ctas) {
-    if (tid == 0) a.records[cta].last = -1;
+  const long long W = plan_build<BK>(a, &s_plan, gridDim.x);
+  Work k;
+  if (!work_begin<BK>(a, &s_plan, W, cta, gridDim.x, k)) {
+    if (tid == 0) leave_record(a, cta, k);
     return;
   }
-  const long long w_lo = shares.begin(cta), w_hi = shares.begin(cta + 1);
-  Cursor cur = plan_locate<BK>(a, &s_plan, w_lo);
-  long long w = w_lo;
 
   while (true) {
-    const int t0 = cur.tile;
-    const int t1 = static_cast<int>(min(static_cast<long long>(cur.tiles), cur.tile + (w_hi - w)));
+    const Cursor& cur = k.cur;
+    const int t0 = k.t0, t1 = k.t1;
     const int kvh = cur.vh / a.nsub, sub = cur.vh % a.nsub;
     const int heads = min(a.gs, a.g - sub * a.gs);
     const int tok0 = cur.qt * a.tq, toks = min(a.tq, cur.s.n - tok0);
@@ -529,10 +526,10 @@ __global__ void __launch_bounds__(128, (MmaCfg<D, MT, BITS4>::CTAS > 2 && MT == 
         }
       }
     __syncthreads();
-    const bool whole = t0 == 0 && t1 == cur.tiles;
-    const long long slot = 2ll * cta + (cur.start > w_lo ? 1 : 0);
+    const bool whole = k.slot < 0;
+    const long long slot = k.slot;
     for (int i = tid; i < R * (D / 8); i += 128) {
-      const int r = i / (D / 8), d = (i % (D / 8)) * 8;
+      const int r = i % R, d = (i / R) * 8;  // (rows innermost: so are the partial results')
       if (!row_ok(r)) continue;
       float top = kNegInf, sum = 0.f;
 #pragma unroll
@@ -566,69 +563,68 @@ __global__ void __launch_bounds__(128, (MmaCfg<D, MT, BITS4>::CTAS > 2 && MT == 
         if (d == 0 && a.lse != nullptr)
           a.lse[tok * (static_cast<long long>(a.c.Hkv) * a.g) + head] = sum == 0.f ? kNegInf : (top + log2f(sum)) * kLn2;
       } else {
-        float4* p = reinterpret_cast<float4*>(a.part_o + (slot * R + r) * D + d);
-        p[0] = make_float4(o[0], o[1], o[2], o[3]);
-        p[1] = make_float4(o[4], o[5], o[6], o[7]);
+        float* p = a.part_o + (slot * D + d) * R + r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e * R] = o[e];
         if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * R + r) * 2) = make_float2(top, sum);
       }
     }
-    w += t1 - t0;
-    if (w >= w_hi) {
-      if (tid == 0) leave_record(a, cta, shares, cur, cur.start >= w_lo && t1 < cur.tiles, w_lo);
-      break;
-    }
-    plan_next<BK>(a, cur);
+    if (k.w + (t1 - t0) >= k.w_hi && tid == 0) leave_record(a, cta, k);
+    if (!work_next<BK>(a, W, cta, gridDim.x, k)) break;
     __syncthreads();  // the merge buffer is the next segment's ring
   }
 }
 
-// Joins the parts of the segments that were cut: CTA c takes the segment that begins in share c
-// and runs past its end (as its record says), a warp one row of it, the parts in the order of their
-// shares.
+// Joins the parts of the segments that were cut: CTA c takes the segment that its record names, a
+// thread one row and 16 dims of it (rows along the lanes, as the parts lie), the parts in the order
+// of their CTAs.
 template <int D, typename T>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ AttnArgs a, int R) {
-  constexpr int V = D / 32;  // floats per lane
   using H = Half2<T>;
+  constexpr int CW = 16;  // dims of a thread
   pdl_wait_prior_grids();
   pdl_launch_dependents();
   const int c = blockIdx.x;
   const JoinRecord rec = a.records[c];
   if (rec.last < 0) return;
-  const int last = rec.last, lane = threadIdx.x & 31;
+  const int last = rec.last, i = blockIdx.y * 128 + threadIdx.x;
+  const int r = i % R, d = (i / R) * CW;
+  if (r >= rec.rows || r % a.gs >= rec.heads || d >= D) return;
   const long long first = rec.slot;
-  for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < rec.rows; r += gridDim.y * 4) {
-    if (r % a.gs >= rec.heads) continue;
-    float top = kNegInf;
-    for (int p = c + lane; p <= last; p += 32)
-      top = fmaxf(top, a.part_ml[((p == c ? first : 2ll * p) * R + r) * 2]);
+  float top = kNegInf, sum = 0.f;
+#pragma unroll 8
+  for (int p = c; p <= last; ++p) top = fmaxf(top, a.part_ml[((p == c ? first : 2ll * p) * R + r) * 2]);
+  float acc[CW];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float acc[V], sum = 0.f;
+  for (int e = 0; e < CW; ++e) acc[e] = 0.f;
+#pragma unroll 2
+  for (int p = c; p <= last; ++p) {
+    const long long at = p == c ? first : 2ll * p;
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (at * R + r) * 2);
+    const float* o = a.part_o + (at * D + d) * R + r;
+    float v[CW];
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] = 0.f;
-#pragma unroll 4
-    for (int p = c; p <= last; ++p) {
-      const long long at = (p == c ? first : 2ll * p) * R + r;
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
-      const float f = ml.x == kNegInf ? 1.f : exp2_fast(ml.x - top);
-      sum = fmaf(ml.y, f, sum);
-      const float* o = a.part_o + at * D + lane * V;
+    for (int e = 0; e < CW; ++e) v[e] = o[e * R];
+    const float f = ml.x == kNegInf ? 1.f : exp2_fast(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
 #pragma unroll
-      for (int e = 0; e < V; e += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(o + e);
-        acc[e] = fmaf(v.x, f, acc[e]);
-        acc[e + 1] = fmaf(v.y, f, acc[e + 1]);
-      }
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const long long tok = rec.tok + r / a.gs;
-    const int head = rec.head + r % a.gs;
-    T* dst = static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + lane * V;
-#pragma unroll
-    for (int e = 0; e < V; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = H::pack(acc[e] * inv, acc[e + 1] * inv);
-    if (lane == 0 && a.lse != nullptr)
-      a.lse[tok * (static_cast<long long>(a.c.Hkv) * a.g) + head] = sum == 0.f ? kNegInf : (top + log2f(sum)) * kLn2;
+    for (int e = 0; e < CW; ++e) acc[e] = fmaf(v[e], f, acc[e]);
   }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const long long tok = rec.tok + r / a.gs;
+  const int head = rec.head + r % a.gs;
+  uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + d);
+#pragma unroll
+  for (int e = 0; e < CW / 8; ++e) {
+    uint4 v;
+    v.x = H::pack(acc[8 * e] * inv, acc[8 * e + 1] * inv);
+    v.y = H::pack(acc[8 * e + 2] * inv, acc[8 * e + 3] * inv);
+    v.z = H::pack(acc[8 * e + 4] * inv, acc[8 * e + 5] * inv);
+    v.w = H::pack(acc[8 * e + 6] * inv, acc[8 * e + 7] * inv);
+    dst[e] = v;
+  }
+  if (d == 0 && a.lse != nullptr)
+    a.lse[tok * (static_cast<long long>(a.c.Hkv) * a.g) + head] = sum == 0.f ? kNegInf : (top + log2f(sum)) * kLn2;
 }
 
 struct Variant {
@@ -704,7 +700,7 @@ cudaError_t launch_attn_join(const AttnArgs& a, const AttnPlan& p, int D, bool b
               : reinterpret_cast<const void*>(paged_join_kernel<256, __half>);
   int R = p.rows;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.grid, (R + 15) / 16);
+  cfg.gridDim = dim3(p.grid, (R * (D / 16) + 127) / 128);
   cfg.blockDim = dim3(128);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

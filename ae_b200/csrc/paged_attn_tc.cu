@@ -48,9 +48,10 @@ template <int D, bool DUAL>
 struct TcCfg {
   static constexpr int R = DUAL ? 256 : 128;
   static constexpr int TILE = kTBK * D * 2;                 // bytes of a K or V tile, and of 128 rows of Q
-  static constexpr int Q = (DUAL ? 2 : 1) * TILE;
-  static constexpr int MERGE = DUAL ? 0 : 128 * 32 * 4;     // 32 columns of the second stream's output
-  static constexpr int SMEM = Q + kTSlots * TILE + MERGE + 1024;
+  // (the single row tile's place also holds the streams' exchange of outputs: 2 x 32 columns)
+  static constexpr int Q = DUAL ? 2 * TILE : TILE > 32768 ? TILE : 32768;
+  static constexpr int SMEM = Q + kTSlots * TILE + 1024;
+  static_assert(DUAL || Q >= 2 * 128 * 32 * 4, "room for the streams' exchange");
 };
 
 // TMEM columns: S of the streams at 0 and 128 (P in their first 64), O at 256 and 384.
@@ -172,19 +173,21 @@ __global__ void __launch_bounds__(kTThreads, 1)
   constexpr int R = C::R, TILE = C::TILE;
   constexpr uint32_t HALF = kTBK * 128;  // bytes of 64 dims of a tile
   extern __shared__ uint8_t dyn_smem[];
-  __shared__ PlanShared s_plan;
   __shared__ uint64_t full_bar[kTSlots], empty_bar[kTSlots], s_bar[2], p_bar[2][2], o_bar[2], q_bar[2], drain_bar, both_bar;
   __shared__ uint64_t seg_full[kTSegs], seg_empty[kTSegs];
   __shared__ Segment s_seg[kTSegs];
   __shared__ uint32_t s_tmem, s_pages[kTOkRing];
   __shared__ int s_abort, s_fix;
-  __shared__ float2 s_ml[DUAL ? 1 : 128];
+  __shared__ float2 s_ml[2][DUAL ? 1 : 128];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t raw = smem_u32(dyn_smem);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* sm = dyn_smem + (base - raw);
   const uint32_t q_s = base, ring_s = base + C::Q;
+  // the plan lies where the ring will be: the first copy into it follows the first segment, and that
+  // follows the last look at the plan
+  PlanShared* plan = reinterpret_cast<PlanShared*>(sm + C::Q);
 
   if (tid == 0) {
     s_abort = 0;
@@ -221,16 +224,12 @@ __global__ void __launch_bounds__(kTThreads, 1)
 
   pdl_wait_prior_grids();
   pdl_launch_dependents();
-  const long long W = plan_build<kTBK>(a, &s_plan);
-  const Shares shares(a, W, gridDim.x);
   const int cta = blockIdx.x;
-  const bool works = W > 0 && cta < shares.ctas;
-  const long long w_lo = works ? shares.begin(cta) : 0, w_hi = works ? shares.begin(cta + 1) : 0;
-  if (!works && tid == 0) a.records[cta].last = -1;
+  const long long W = plan_build<kTBK>(a, plan, gridDim.x);
   int* status = a.status;
   volatile int* abort_flag = &s_abort;
 
-  if (works) {
+  {
     // The i-th segment of the share; false when it is done, or after a failed wait.
     auto next_segment = [&](int i, Segment& g) {
       if (!mbar_wait(&seg_full[i % kTSegs], (i / kTSegs) & 1, status, abort_flag)) return false;
@@ -295,11 +294,15 @@ __global__ void __launch_bounds__(kTThreads, 1)
           mbar_wait(&full_bar[i % kTSlots], (i / kTSlots) & 1, status, nullptr);
       } else if (warp == 3 && lane == 0) {
         // ---------------------------------------------------------------- segments
-        Cursor cur = plan_locate<kTBK>(a, &s_plan, w_lo);
-        for (long long w = w_lo; w < w_hi; ++seg) {
+        Work k;
+        bool more = work_begin<kTBK>(a, plan, W, cta, gridDim.x, k);
+        if (!more) leave_record(a, cta, k);
+        while (more) {
+          const Cursor& cur = k.cur;
           Segment n;
-          n.t0 = cur.tile;
-          n.t1 = static_cast<int>(min(static_cast<long long>(cur.tiles), cur.tile + (w_hi - w)));
+          n.t0 = k.t0;
+          n.t1 = k.t1;
+          n.slot = k.slot;
           n.keys = cur.keys;
           const int sub = cur.vh % a.nsub;
           n.kvh = cur.vh / a.nsub;
@@ -311,15 +314,12 @@ __global__ void __launch_bounds__(kTThreads, 1)
           n.toks = min(a.tq, cur.s.n - n.i0);
           n.prefix = cur.s.L - cur.s.n;
           n.open = a.tree != nullptr ? n.prefix : n.prefix + n.i0 + 1;
-          n.slot = n.t0 == 0 && n.t1 == cur.tiles ? -1 : 2 * cta + (cur.start > w_lo ? 1 : 0);
           mbar_wait(&seg_empty[seg % kTSegs], ((seg / kTSegs) & 1) ^ 1, status, abort_flag);
           s_seg[seg % kTSegs] = n;
           mbar_arrive(&seg_full[seg % kTSegs]);
-          w += n.t1 - n.t0;
-          if (w >= w_hi)
-            leave_record(a, cta, shares, cur, cur.start >= w_lo && n.t1 < cur.tiles, w_lo);
-          else
-            plan_next<kTBK>(a, cur);
+          ++seg;
+          if (k.w + (k.t1 - k.t0) >= k.w_hi) leave_record(a, cta, k);
+          more = work_next<kTBK>(a, W, cta, gridDim.x, k);
         }
         mbar_wait(&seg_empty[seg % kTSegs], ((seg / kTSegs) & 1) ^ 1, status, abort_flag);
         s_seg[seg % kTSegs].t1 = -1;
@@ -610,25 +610,22 @@ __global__ void __launch_bounds__(kTThreads, 1)
         }
         const bool whole = g.slot < 0;
         const long long slot = g.slot;
-        float f0 = 1.f, f1 = 0.f;
+        float f_own = 1.f, f_other = 0.f;
         if constexpr (!DUAL) {
-          if (s == 1) s_ml[row] = make_float2(m, l);
+          s_ml[s][row] = make_float2(m, l);
           both();
-          if (s == 0) {
-            const float2 o = s_ml[row];
-            const float mx = fmaxf(m, o.x);
-            f0 = m == kNegInf ? 1.f : exp2_fast(m - mx);
-            f1 = o.x == kNegInf ? 1.f : exp2_fast(o.x - mx);
-            l = l * f0 + o.y * f1;
-            m = mx;
-          }
+          const float2 o = s_ml[s ^ 1][row];
+          const float mx = fmaxf(m, o.x);
+          // a stream with no visible key has a maximum of -inf and an output of 0
+          f_own = m == kNegInf ? 1.f : exp2_fast(m - mx);
+          f_other = o.x == kNegInf ? 1.f : exp2_fast(o.x - mx);
+          l = s == 0 ? l * f_own + o.y * f_other : o.y * f_other + l * f_own;
+          m = mx;
         }
         const bool fix = *reinterpret_cast<volatile int*>(&s_fix) != 0;
         float inv = 1.f;
         if (whole) inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t o[32];
+        auto load_o = [&](int q, uint32_t (&o)[32]) {  // 32 columns of this stream's output
           __syncwarp();
           if (mine) {
             tmem_ld32_issue(t_o + q * 32, o);
@@ -656,38 +653,56 @@ __global__ void __launch_bounds__(kTThreads, 1)
               }
             }
           }
-          if constexpr (!DUAL) {
-            float* merge = reinterpret_cast<float*>(sm + C::Q + kTSlots * TILE);
-            if (s == 1) {
+          __syncwarp();
+        };
+        auto store_o = [&](int q, const uint32_t (&o)[32]) {
+          if (!row_ok) return;
+          if (whole) {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + q * 32);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) merge[e * 128 + row] = __uint_as_float(o[e]);
+            for (int c = 0; c < 4; ++c) {
+              uint4 v;
+              v.x = H::pack(__uint_as_float(o[8 * c]) * inv, __uint_as_float(o[8 * c + 1]) * inv);
+              v.y = H::pack(__uint_as_float(o[8 * c + 2]) * inv, __uint_as_float(o[8 * c + 3]) * inv);
+              v.z = H::pack(__uint_as_float(o[8 * c + 4]) * inv, __uint_as_float(o[8 * c + 5]) * inv);
+              v.w = H::pack(__uint_as_float(o[8 * c + 6]) * inv, __uint_as_float(o[8 * c + 7]) * inv);
+              dst[c] = v;
             }
-            __syncwarp();
-            both();
-            if (s == 0) {
+          } else {
+            float* dst = a.part_o + (slot * D + q * 32) * R + r;  // rows innermost: a warp's store is one line
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                o[e] = __float_as_uint(__uint_as_float(o[e]) * f0 + merge[e * 128 + row] * f1);
-            }
-            both();  // the next columns go to the same place
+            for (int e = 0; e < 32; ++e) dst[e * R] = __uint_as_float(o[e]);
           }
-          if ((DUAL || s == 0) && row_ok) {
-            if (whole) {
-              uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + q * 32);
+        };
+        if constexpr (DUAL) {
+#pragma unroll 1
+          for (int q = 0; q < D / 32; ++q) {
+            uint32_t o[32];
+            load_o(q, o);
+            store_o(q, o);
+          }
+        } else {
+          // each stream finishes half of the columns: it leaves 32 of the other's columns at a time where Q
+          // was (every product with Q is complete), [column][row]
+          constexpr int HQ = D / 64;
+          float* give = reinterpret_cast<float*>(sm) + s * (32 * 128);
+          const float* take = reinterpret_cast<const float*>(sm) + (s ^ 1) * (32 * 128);
+#pragma unroll 1
+          for (int q = 0; q < HQ; ++q) {
+            uint32_t o[32];
+            load_o((s ^ 1) * HQ + q, o);
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                uint4 v;
-                v.x = H::pack(__uint_as_float(o[8 * c]) * inv, __uint_as_float(o[8 * c + 1]) * inv);
-                v.y = H::pack(__uint_as_float(o[8 * c + 2]) * inv, __uint_as_float(o[8 * c + 3]) * inv);
-                v.z = H::pack(__uint_as_float(o[8 * c + 4]) * inv, __uint_as_float(o[8 * c + 5]) * inv);
-                v.w = H::pack(__uint_as_float(o[8 * c + 6]) * inv, __uint_as_float(o[8 * c + 7]) * inv);
-                dst[c] = v;
-              }
-            } else {
-              uint4* dst = reinterpret_cast<uint4*>(a.part_o + (slot * R + r) * D + q * 32);
+            for (int e = 0; e < 32; ++e) give[e * 128 + row] = __uint_as_float(o[e]) * f_own;
+            both();
+            load_o(s * HQ + q, o);
 #pragma unroll
-              for (int c = 0; c < 8; ++c) dst[c] = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+            for (int e = 0; e < 32; ++e) {
+              // (the sum in the streams' order on both sides)
+              const float own = __uint_as_float(o[e]) * f_own, other = take[e * 128 + row];
+              o[e] = __float_as_uint(s == 0 ? own + other : other + own);
             }
+            store_o(s * HQ + q, o);
+            if (q + 1 < HQ) both();
           }
         }
         if ((DUAL || s == 0) && row_ok) {
@@ -700,8 +715,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
         tc_fence_before();
         it += 2 * n;
         tc += n;
-        __syncwarp();
-        if constexpr (!DUAL) both();  // both streams are done with Q and (m, l)
+        if constexpr (!DUAL) both();  // both streams are done with Q's place and (m, l)
       }
     }
   }

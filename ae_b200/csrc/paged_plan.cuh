@@ -2,14 +2,20 @@
 // the device (the host does not know them).
 //
 // A segment is (sequence b, key head or part of one vh, row tile qt): the rows of tq tokens x gs
-// query heads against the keys those tokens can see, in tiles of BK keys.  The tiles of all
-// segments in the order (b, vh, qt, tile) form one line of W tiles, and CTA c takes the tiles
-// [W c / G, W (c + 1) / G): whatever the lengths, the CTAs' shares differ by one tile.  A segment
-// that lies inside one share is finished by its CTA; one that is cut leaves a partial result in
-// at most two slots per CTA (2c: the segment its share begins in, 2c + 1: the one it ends in),
-// and a second kernel joins the parts in the order of their CTAs, so the result does not depend
-// on timing.  The slots' size follows the grid and not the lengths.  The CTA in whose share a cut
-// segment begins leaves a record of it, so the second kernel plans nothing.
+// query heads against the keys those tokens can see, in tiles of BK keys.  Two ways to share the
+// segments out, both balanced whatever the lengths:
+//  - pieces, where there are few: every segment of t tiles is cut into ceil(t / T) pieces of equal
+//    length, one CTA each, with T the least number of tiles for which the pieces fit the grid (and no
+//    less than min_tiles: a shorter piece costs more in its start and its join than it saves).  A CTA
+//    has one segment to start and to finish, which is what a short call spends its time on.
+//  - the line, where T would exceed an even share by more than a few tiles: the tiles of all segments
+//    in the order (b, vh, qt, tile) form a line of W tiles, of which CTA c takes the c-th part; the
+//    parts' lengths differ by one tile.
+// A segment that one CTA has to itself is finished there.  One that is cut leaves a partial result in
+// at most two slots per CTA (2c, and on the line 2c + 1 for the segment a share ends in), and a
+// second kernel joins the parts in the order of their CTAs, so the result does not depend on timing.
+// The slots' size follows the grid and not the lengths.  The CTA with the first part of a cut segment
+// leaves a record of it, so the second kernel plans nothing.
 #pragma once
 
 #include "common.cuh"
@@ -98,10 +104,13 @@ __device__ __forceinline__ long long tiles_before(const AttnArgs& a, const Seq& 
   return sum;
 }
 
-// Sums of the sequences before each of kPlanThreads runs of consecutive sequences.
+// Sums over the sequences before each of kPlanThreads runs of consecutive sequences.
 struct PlanShared {
-  long long before[kPlanThreads + 1];
+  long long before[kPlanThreads + 1];  // tiles (line) or pieces
   long long warp_sum[kPlanThreads / 32];
+  Seq seq[kPlanThreads];               // one run, one sequence: up to kPlanThreads sequences
+  int fit[kPlanThreads / 32][4];
+  int piece;                           // T, 0: the line
 };
 
 struct Cursor {
@@ -117,15 +126,11 @@ __device__ __forceinline__ long long seq_tiles(const AttnArgs& a, const Seq& s) 
   return tiles_before<BK>(a, s, row_tiles(a, s)) * (a.c.Hkv * a.nsub);
 }
 
-// Every thread of the CTA calls it; the first kPlanThreads do the work.  Returns W.
-template <int BK>
-__device__ long long plan_build(const AttnArgs& a, PlanShared* sh) {
-  const int per = (a.B + kPlanThreads - 1) / kPlanThreads;
+// Exclusive prefix sums of v over the first kPlanThreads threads into sh->before; every thread calls.
+__device__ __forceinline__ void plan_scan(PlanShared* sh, long long v) {
   const int t = threadIdx.x;
-  long long v = 0, inc = 0;
+  long long inc = v;
   if (t < kPlanThreads) {
-    for (int b = t * per; b < min(a.B, (t + 1) * per); ++b) v += seq_tiles<BK>(a, seq_at(a, b));
-    inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long up = __shfl_up_sync(0xffffffffu, inc, o);
@@ -143,23 +148,84 @@ __device__ long long plan_build(const AttnArgs& a, PlanShared* sh) {
     if (t == kPlanThreads - 1) sh->before[kPlanThreads] = add + inc;
   }
   __syncthreads();
-  return sh->before[kPlanThreads];
 }
 
-// Position of tile w of the line (0 <= w < W).  Uniform over the CTA.
+// The i-th piece length to try, for an even share of `even` tiles.
+__device__ __forceinline__ int piece_length(const AttnArgs& a, long long even, int i) {
+  return static_cast<int>(max(even, static_cast<long long>(a.min_tiles))) + (i == 0 ? 0 : 1 << i);
+}
+__device__ __forceinline__ int pieces_of(int tiles, int T) { return (tiles + T - 1) / T; }
+
+// Every thread of the CTA calls it; the first kPlanThreads do the work.  Returns the tiles W of the
+// line.
 template <int BK>
-__device__ Cursor plan_locate(const AttnArgs& a, const PlanShared* sh, long long w) {
-  int lo = 0, hi = kPlanThreads;  // the last run that starts at or before w
+__device__ long long plan_build(const AttnArgs& a, PlanShared* sh, int grid) {
+  const int per = (a.B + kPlanThreads - 1) / kPlanThreads;
+  const int t = threadIdx.x;
+  long long v = 0;
+  bool single = per == 1;  // every sequence has a run of its own and at most one row tile
+  Seq s{0, 0, 0};
+  if (t < kPlanThreads) {
+    for (int b = t * per; b < min(a.B, (t + 1) * per); ++b) {
+      s = seq_at(a, b);
+      v += seq_tiles<BK>(a, s);
+      single = single && s.n <= a.tq;
+    }
+    sh->seq[t] = s;
+  }
+  plan_scan(sh, v);
+  const long long W = sh->before[kPlanThreads];
+  const long long even = quotient(W + grid - 1, grid);
+  if (t == 0) sh->piece = 0;
+  if (!__syncthreads_and(single) || W == 0 || even > 0x3fffffff) return W;
+  const int Hv = a.c.Hkv * a.nsub;
+  const int tiles = t < kPlanThreads && s.n > 0 ? tiles_of<BK>(keys_of_tile(a, s, 0)) : 0;
+  if (t < kPlanThreads) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // (sums that matter are at most the grid's size)
+      int n = min(pieces_of(tiles, piece_length(a, even, i)), 1 << 12) * Hv;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+      if ((t & 31) == 0) sh->fit[t >> 5][i] = n;
+    }
+  }
+  __syncthreads();
+  int T = 0;
+#pragma unroll
+  for (int i = 3; i >= 0; --i) {
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 32; ++w) n += sh->fit[w][i];
+    if (n <= grid) T = piece_length(a, even, i);
+  }
+  if (T > 0) {  // (uniform)
+    if (t == 0) sh->piece = T;
+    plan_scan(sh, static_cast<long long>(tiles > 0 ? pieces_of(tiles, T) * Hv : 0));
+  }
+  return W;
+}
+
+// The last run that starts at or before w.
+__device__ __forceinline__ int plan_run(const PlanShared* sh, long long w) {
+  int lo = 0, hi = kPlanThreads;
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
     if (sh->before[mid] <= w) lo = mid;
     else hi = mid;
   }
+  return lo;
+}
+
+// Position of tile w of the line (0 <= w < W).
+template <int BK>
+__device__ Cursor plan_locate(const AttnArgs& a, const PlanShared* sh, long long w) {
   const int per = (a.B + kPlanThreads - 1) / kPlanThreads;
-  long long at = sh->before[lo];
+  const int run = plan_run(sh, w);
+  long long at = sh->before[run];
   Cursor c;
-  c.b = lo * per;
-  c.s = seq_at(a, c.b);
+  c.b = run * per;
+  c.s = per == 1 ? sh->seq[run] : seq_at(a, c.b);
   for (int i = 1; i < per && c.b + 1 < a.B; ++i) {  // w < W, so a sequence that holds it comes before B
     const long long here = seq_tiles<BK>(a, c.s);
     if (w < at + here) break;
@@ -204,8 +270,8 @@ __device__ __forceinline__ void plan_next(const AttnArgs& a, Cursor& c) {
   c.tiles = tiles_of<BK>(c.keys);
 }
 
-// The shares: CTA c of `ctas` takes [begin(c), begin(c + 1)), the first `more` one tile more than the
-// others.  No share is below min_tiles while that leaves CTAs idle.
+// The line's shares: CTA c of `ctas` takes [begin(c), begin(c + 1)), the first `more` one tile more
+// than the others.  No share is below min_tiles while that leaves CTAs idle.
 struct Shares {
   long long each;
   int more, ctas;
@@ -221,15 +287,71 @@ struct Shares {
   }
 };
 
-// Notes for the join, by the CTA whose share ends with (c, t1): `first` = it is the segment's first
-// part and others follow.  Called by one thread, once.
-__device__ __forceinline__ void leave_record(const AttnArgs& a, int cta, const Shares& sh, const Cursor& c, bool cut,
-                                             long long w_lo) {
+// The segments of one CTA, one after the other.
+struct Work {
+  Cursor cur;
+  int t0, t1;     // key tiles of the segment that are this CTA's
+  int slot;       // where its partial result goes, -1: the segment is this CTA's alone
+  int last;       // last CTA with a part of it, if this one has the first of several; -1 otherwise
+  long long w, w_lo, w_hi;
+};
+
+__device__ __forceinline__ void work_open(const Shares& sh, int cta, Work& k) {
+  k.t0 = k.cur.tile;
+  k.t1 = static_cast<int>(min(static_cast<long long>(k.cur.tiles), k.t0 + (k.w_hi - k.w)));
+  const bool whole = k.t0 == 0 && k.t1 == k.cur.tiles;
+  k.slot = whole ? -1 : 2 * cta + (k.cur.start > k.w_lo ? 1 : 0);
+  k.last = k.t0 == 0 && !whole ? sh.owner(k.cur.start + k.cur.tiles - 1) : -1;
+}
+
+// This CTA's first segment; false if it has none.
+template <int BK>
+__device__ bool work_begin(const AttnArgs& a, const PlanShared* sh, long long W, int cta, int grid, Work& k) {
+  k.last = -1;
+  if (sh->piece > 0) {
+    if (cta >= sh->before[kPlanThreads]) return false;
+    k.cur.b = plan_run(sh, cta);
+    k.cur.s = sh->seq[k.cur.b];
+    k.cur.qt = 0;
+    k.cur.keys = keys_of_tile(a, k.cur.s, 0);
+    k.cur.tiles = tiles_of<BK>(k.cur.keys);
+    const int pieces = pieces_of(k.cur.tiles, sh->piece), i = static_cast<int>(cta - sh->before[k.cur.b]);
+    k.cur.vh = i / pieces;
+    const int p = i % pieces, len = k.cur.tiles / pieces, more = k.cur.tiles % pieces;
+    k.t0 = p * len + min(p, more);
+    k.t1 = k.t0 + len + (p < more);
+    k.slot = pieces == 1 ? -1 : 2 * cta;
+    if (p == 0 && pieces > 1) k.last = cta + pieces - 1;
+    k.w = k.w_hi = 0;
+    return true;
+  }
+  const Shares line(a, W, grid);
+  if (W == 0 || cta >= line.ctas) return false;
+  k.w_lo = line.begin(cta);
+  k.w_hi = line.begin(cta + 1);
+  k.w = k.w_lo;
+  k.cur = plan_locate<BK>(a, sh, k.w);
+  work_open(line, cta, k);
+  return true;
+}
+
+template <int BK>
+__device__ __forceinline__ bool work_next(const AttnArgs& a, long long W, int cta, int grid, Work& k) {
+  k.w += k.t1 - k.t0;
+  if (k.w >= k.w_hi) return false;
+  plan_next<BK>(a, k.cur);
+  work_open(Shares(a, W, grid), cta, k);
+  return true;
+}
+
+// Notes for the join: called by one thread for the CTA's last segment (the only one that others may
+// go on with), or with none.
+__device__ __forceinline__ void leave_record(const AttnArgs& a, int cta, const Work& k) {
   JoinRecord r;
-  r.last = -1;
-  if (cut) {
-    r.last = sh.owner(c.start + c.tiles - 1);
-    r.slot = 2 * cta + (c.start > w_lo ? 1 : 0);
+  r.last = k.last;
+  if (k.last >= 0) {
+    const Cursor& c = k.cur;
+    r.slot = k.slot;
     const int kvh = c.vh / a.nsub, sub = c.vh % a.nsub;
     r.heads = min(a.gs, a.g - sub * a.gs);
     r.head = kvh * a.g + sub * a.gs;
