@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -19,7 +20,6 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
 _S = ctypes.c_size_t
-_F = ctypes.c_float
 SIGNATURES = {
     "smb_version": (_I, []),
     "smb_strerror": (ctypes.c_char_p, [_I]),
@@ -63,21 +63,18 @@ SIGNATURES = {
     "smb_moe_read_timers": (_I, [_P, _S, _I, _P, _P]),
     "smb_moe_noalloc_read_status": (_I, [_P]),
     "smb_kv4_row_bytes": (_I, [_I]),
-    "smb_kv_append": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _F, _P, _P, _F, _P, _P, _P]),
-    "smb_kv4_read": (_I, [_P, _L, _I, _I, _I, _L, _L, _L, _I, _P, _I, _P, _P]),
+    "smb_kv_append": (_I, [ctypes.c_char_p, _P]),
+    "smb_kv4_read": (_I, [ctypes.c_char_p, _I, _P, _I, _P, _P]),
     "smb_paged_attention_workspace_bytes": (_S, [_I, _I, _I, _I, _I, _I]),
-    "smb_paged_attention": (_I, [_P, _P, _L, _L, _I, _I, _I, _I, _P, _L, _I, _P, _P, _P, _L, _I, _F, _P, _L, _L,
-                                 _P, _P, _P, _S, _P]),
+    "smb_paged_attention": (_I, [ctypes.c_char_p, _P]),
 }
 
-
-class PagedCache(ctypes.Structure):
-    """``smb_paged_cache_t`` of ``include/ae_b200.h``: one layer's paged key/value cache."""
-
-    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("num_pages", ctypes.c_int64),
-                ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64),
-                ("kv_heads", ctypes.c_int), ("page_size", ctypes.c_int), ("head_dim", ctypes.c_int),
-                ("bits", ctypes.c_int)]
+# The argument structs of the paged cache (include/ae_b200.h), as formats of the struct module: one
+# pack and one pointer cost a call less than a ctypes argument for each field.
+PAGED_CACHE = "PPqqqqiiii"
+APPEND_ARGS = struct.Struct("N" + PAGED_CACHE + "PPP6qPPPPPPPiiiiiff0P")
+ATTENTION_ARGS = struct.Struct("N" + PAGED_CACHE + "PqqPqqPqPPPqPPPNiiiiiif0P")
+CACHE_ARGS = struct.Struct(PAGED_CACHE)
 
 
 class Timers(ctypes.Structure):

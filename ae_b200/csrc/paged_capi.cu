@@ -63,66 +63,59 @@ int smb_kv4_row_bytes(int head_dim) {
   return kv4_row_bytes(head_dim);
 }
 
-int smb_kv_append(const smb_paged_cache_t* cache, const void* q, const void* k, const void* v, const int64_t* strides,
-                  int dtype, int N, int Hq, const int64_t* slots, const int64_t* positions, const double* inv_freq,
-                  int rot, int interleaved, float rope_scale, const void* q_norm, const void* k_norm, float eps,
-                  void* q_out, int* status, smb_stream_t stream) {
+int smb_kv_append(const smb_append_args_t* p, smb_stream_t stream) {
+  if (p == nullptr) return SMB_ERR_NULL;
+  if (p->struct_bytes != sizeof(*p)) return SMB_ERR_SHAPE;
   AppendArgs a{};
-  int rc = cache_args(cache, &a.c);
+  int rc = cache_args(&p->cache, &a.c);
   if (rc != SMB_OK) return rc;
-  if (!storage(dtype)) return SMB_ERR_DTYPE;
-  const int D = cache->head_dim;
+  if (!storage(p->dtype)) return SMB_ERR_DTYPE;
+  const int D = p->cache.head_dim, N = p->N, Hq = p->Hq, rot = p->rot;
   if (N < 0 || Hq < 1 || Hq > kPagedMaxHeads || rot < 0 || rot > D || rot % 16 != 0) return SMB_ERR_SHAPE;
   if (N == 0) return SMB_OK;
-  if (q == nullptr || k == nullptr || v == nullptr || strides == nullptr || slots == nullptr || q_out == nullptr)
+  if (p->q == nullptr || p->k == nullptr || p->v == nullptr || p->slots == nullptr || p->q_out == nullptr)
     return SMB_ERR_NULL;
-  if (rot > 0 && (positions == nullptr || inv_freq == nullptr)) return SMB_ERR_NULL;
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(q_norm) || !aligned16(k_norm))
+  if (rot > 0 && (p->positions == nullptr || p->inv_freq == nullptr)) return SMB_ERR_NULL;
+  if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->q_out) || !aligned16(p->q_norm) ||
+      !aligned16(p->k_norm))
     return SMB_ERR_ALIGN;
-  for (int i = 0; i < 6; ++i)
-    if (strides[i] % 8 != 0) return SMB_ERR_ALIGN;
+  for (int i = 0; i < 2; ++i)
+    if (p->q_strides[i] % 8 != 0 || p->k_strides[i] % 8 != 0 || p->v_strides[i] % 8 != 0) return SMB_ERR_ALIGN;
   DeviceInfo di;
   rc = need_b200(&di);
   if (rc != SMB_OK) return rc;
-  a.q = q;
-  a.k = k;
-  a.v = v;
-  a.q_ts = strides[0];
-  a.q_hs = strides[1];
-  a.k_ts = strides[2];
-  a.k_hs = strides[3];
-  a.v_ts = strides[4];
-  a.v_hs = strides[5];
-  a.slots = reinterpret_cast<const long long*>(slots);
-  a.positions = reinterpret_cast<const long long*>(positions);
-  a.inv_freq = inv_freq;
+  a.q = p->q;
+  a.k = p->k;
+  a.v = p->v;
+  a.q_ts = p->q_strides[0];
+  a.q_hs = p->q_strides[1];
+  a.k_ts = p->k_strides[0];
+  a.k_hs = p->k_strides[1];
+  a.v_ts = p->v_strides[0];
+  a.v_hs = p->v_strides[1];
+  a.slots = reinterpret_cast<const long long*>(p->slots);
+  a.positions = reinterpret_cast<const long long*>(p->positions);
+  a.inv_freq = p->inv_freq;
   a.rot = rot;
-  a.interleaved = interleaved;
-  a.rope_scale = rope_scale;
-  a.eps = eps;
-  a.q_norm = q_norm;
-  a.k_norm = k_norm;
-  a.q_out = q_out;
-  a.status = status;
+  a.interleaved = p->interleaved;
+  a.rope_scale = p->rope_scale;
+  a.eps = p->eps;
+  a.q_norm = p->q_norm;
+  a.k_norm = p->k_norm;
+  a.q_out = p->q_out;
+  a.status = p->status;
   a.N = N;
   a.Hq = Hq;
-  return done(launch_kv_append(a, D, dtype == SMB_DTYPE_BF16, cache->bits == 4, di.sms,
+  return done(launch_kv_append(a, D, p->dtype == SMB_DTYPE_BF16, p->cache.bits == 4, di.sms,
                                reinterpret_cast<cudaStream_t>(stream), pdl_enabled()));
 }
 
-int smb_kv4_read(const void* cache, int64_t num_pages, int kv_heads, int page_size, int head_dim, int64_t page_stride,
-                 int64_t head_stride, int64_t token_stride, int dtype, const int64_t* slots, int M, void* out,
+int smb_kv4_read(const smb_paged_cache_t* cache, int dtype, const int64_t* slots, int M, void* out,
                  smb_stream_t stream) {
-  smb_paged_cache_t c{};
-  c.k = c.v = const_cast<void*>(cache);
-  c.num_pages = num_pages;
-  c.page_stride = page_stride;
-  c.head_stride = head_stride;
-  c.token_stride = token_stride;
-  c.kv_heads = kv_heads;
-  c.page_size = page_size;
-  c.head_dim = head_dim;
-  c.bits = 4;
+  if (cache == nullptr) return SMB_ERR_NULL;
+  smb_paged_cache_t c = *cache;
+  c.v = c.k;
+  if (c.bits != 4) return SMB_ERR_DTYPE;
   PagedCacheArgs ca;
   int rc = cache_args(&c, &ca);
   if (rc != SMB_OK) return rc;
@@ -145,7 +138,7 @@ int smb_kv4_read(const void* cache, int64_t num_pages, int kv_heads, int page_si
   a.slots = reinterpret_cast<const long long*>(slots);
   a.M = M;
   a.out = out;
-  return done(launch_kv4_read(a, head_dim, dtype == SMB_DTYPE_BF16, reinterpret_cast<cudaStream_t>(stream), pdl_enabled()));
+  return done(launch_kv4_read(a, c.head_dim, dtype == SMB_DTYPE_BF16, reinterpret_cast<cudaStream_t>(stream), pdl_enabled()));
 }
 
 size_t smb_paged_attention_workspace_bytes(int N, int B, int Hq, int Hkv, int head_dim, int bits) {
@@ -161,62 +154,62 @@ size_t smb_paged_attention_workspace_bytes(int N, int B, int Hq, int Hkv, int he
   return n;
 }
 
-int smb_paged_attention(const smb_paged_cache_t* cache, const void* q, int64_t q_token_stride, int64_t q_head_stride,
-                        int dtype, int N, int Hq, int B, const int32_t* block_table, int64_t table_stride,
-                        int max_pages, const int32_t* kv_lens, const int32_t* q_starts, const int32_t* tree,
-                        int64_t tree_stride, int tree_words, float scale, void* out, int64_t out_token_stride,
-                        int64_t out_head_stride, float* lse, int* status, void* ws, size_t ws_bytes,
-                        smb_stream_t stream) {
+int smb_paged_attention(const smb_attention_args_t* r, smb_stream_t stream) {
+  if (r == nullptr) return SMB_ERR_NULL;
+  if (r->struct_bytes != sizeof(*r)) return SMB_ERR_SHAPE;
   AttnArgs a{};
-  int rc = cache_args(cache, &a.c);
+  int rc = cache_args(&r->cache, &a.c);
   if (rc != SMB_OK) return rc;
-  if (!storage(dtype)) return SMB_ERR_DTYPE;
-  const int D = cache->head_dim;
-  rc = attn_sizes(N, B, Hq, a.c.Hkv, D, cache->bits);
+  if (!storage(r->dtype)) return SMB_ERR_DTYPE;
+  const int D = r->cache.head_dim, N = r->N, B = r->B;
+  rc = attn_sizes(N, B, r->Hq, a.c.Hkv, D, r->cache.bits);
   if (rc != SMB_OK) return rc;
-  if (max_pages < 0 || table_stride < 0 || (tree != nullptr && (tree_words < 1 || tree_stride < 0))) return SMB_ERR_SHAPE;
-  if (!(scale > 0.f) || scale > 1e30f) return SMB_ERR_SHAPE;
+  if (r->max_pages < 0 || r->table_stride < 0) return SMB_ERR_SHAPE;
+  if (r->tree != nullptr && (r->tree_words < 1 || r->tree_stride < 0)) return SMB_ERR_SHAPE;
+  if (!(r->scale > 0.f) || r->scale > 1e30f) return SMB_ERR_SHAPE;
   if (N == 0 || B == 0) return SMB_OK;
-  if (q == nullptr || out == nullptr || kv_lens == nullptr || q_starts == nullptr || ws == nullptr) return SMB_ERR_NULL;
-  if (max_pages > 0 && block_table == nullptr) return SMB_ERR_NULL;
-  if (!aligned16(q) || !aligned16(out) || !aligned16(ws)) return SMB_ERR_ALIGN;
-  if (q_token_stride % 8 || q_head_stride % 8 || out_token_stride % 8 || out_head_stride % 8) return SMB_ERR_ALIGN;
+  if (r->q == nullptr || r->out == nullptr || r->kv_lens == nullptr || r->q_starts == nullptr || r->ws == nullptr)
+    return SMB_ERR_NULL;
+  if (r->max_pages > 0 && r->block_table == nullptr) return SMB_ERR_NULL;
+  if (!aligned16(r->q) || !aligned16(r->out) || !aligned16(r->ws)) return SMB_ERR_ALIGN;
+  for (int i = 0; i < 2; ++i)
+    if (r->q_strides[i] % 8 != 0 || r->out_strides[i] % 8 != 0) return SMB_ERR_ALIGN;
   DeviceInfo di;
   rc = need_b200(&di);
   if (rc != SMB_OK) return rc;
-  a.q = q;
-  a.q_ts = q_token_stride;
-  a.q_hs = q_head_stride;
+  a.q = r->q;
+  a.q_ts = r->q_strides[0];
+  a.q_hs = r->q_strides[1];
   a.N = N;
   a.B = B;
-  a.g = Hq / a.c.Hkv;
-  a.table = block_table;
-  a.table_stride = table_stride;
-  a.max_pages = max_pages;
-  a.kv_lens = kv_lens;
-  a.q_starts = q_starts;
-  a.tree = tree;
-  a.tree_stride = tree_stride;
-  a.tree_words = tree_words;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.out = out;
-  a.o_ts = out_token_stride;
-  a.o_hs = out_head_stride;
-  a.lse = lse;
-  a.status = status;
-  const bool bits4 = cache->bits == 4;
+  a.g = r->Hq / a.c.Hkv;
+  a.table = r->block_table;
+  a.table_stride = r->table_stride;
+  a.max_pages = r->max_pages;
+  a.kv_lens = r->kv_lens;
+  a.q_starts = r->q_starts;
+  a.tree = r->tree;
+  a.tree_stride = r->tree_stride;
+  a.tree_words = r->tree_words;
+  a.scale_log2 = r->scale * 1.4426950408889634f;
+  a.out = r->out;
+  a.o_ts = r->out_strides[0];
+  a.o_hs = r->out_strides[1];
+  a.lse = r->lse;
+  a.status = r->status;
+  const bool bits4 = r->cache.bits == 4;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const bool bf16 = dtype == SMB_DTYPE_BF16;
+  const bool bf16 = r->dtype == SMB_DTYPE_BF16;
   AttnPlan p;
   auto use = [&]() {
     a.gs = std::min(a.g, p.rows);
     a.nsub = (a.g + a.gs - 1) / a.gs;
     a.tq = p.rows / a.gs;
-    a.part_o = static_cast<float*>(ws);
+    a.part_o = static_cast<float*>(r->ws);
     a.part_ml = a.part_o + static_cast<size_t>(2) * p.grid * p.rows * D;
     a.records = reinterpret_cast<JoinRecord*>(a.part_ml + static_cast<size_t>(4) * p.grid * p.rows);
     a.min_tiles = 2;
-    return ws_bytes >= attn_ws(p, D);
+    return r->ws_bytes >= attn_ws(p, D);
   };
   if (tc_takes(a.c) && plan_attn_tc(N, B, a.g, D, bits4, di.sms, &p)) {
     if (!use()) return SMB_ERR_WORKSPACE;

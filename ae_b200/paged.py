@@ -21,14 +21,13 @@ Everything is for inference (no gradients) and runs on the current stream of the
 """
 from __future__ import annotations
 
-import ctypes
+import functools
 import math
 from typing import List, Optional, Sequence, Tuple
 
 import torch
 
 from . import _native, ops
-from .ops import _STORAGE, _stream_ptr
 
 HEAD_DIMS = (64, 128, 256)
 
@@ -125,70 +124,71 @@ def tree_words(parents: Sequence[List[int]]) -> torch.Tensor:
     return torch.cat(rows) if rows else torch.zeros(0, 1, dtype=torch.int32)
 
 
-def _cache(k: torch.Tensor, v: torch.Tensor, head_dim: int, dtype: torch.dtype, dev: torch.device):
-    """The C description of a cache, checked."""
+def _cache(k: torch.Tensor, v: torch.Tensor, head_dim: int, dtype: torch.dtype, dev: int):
+    """The fields of the C description of a cache (``smb_paged_cache_t``), checked."""
     if head_dim not in HEAD_DIMS:
         raise NotImplementedError(f"head_dim {head_dim} (supported: {HEAD_DIMS})")
-    if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
+    shape, stride, kind = k.shape, k.stride(), k.dtype
+    if len(shape) != 4 or v.shape != shape or v.stride() != stride or v.dtype != kind:
         raise ValueError("k_cache and v_cache must be [num_pages, kv_heads, page_size, row] of one dtype and "
                          "with the same strides")
-    if k.device != dev or v.device != dev:
+    if k.get_device() != dev or v.get_device() != dev:
         raise ValueError("the cache must be on the device of the other tensors")
-    pages, heads, size, row = k.shape
-    if k.dtype == torch.uint8:
-        bits, want, elem = 4, kv4_row_bytes(head_dim), 1
-    elif k.dtype == dtype:
-        bits, want, elem = 16, head_dim, 2
+    pages, heads, size, row = shape
+    ps, hs, ts, es = stride
+    if kind == dtype:
+        bits, want = 16, head_dim
+        ps, hs, ts = 2 * ps, 2 * hs, 2 * ts
+    elif kind == torch.uint8:
+        bits, want = 4, kv4_row_bytes(head_dim)
     else:
-        raise ValueError(f"cache dtype {k.dtype} is neither {dtype} nor uint8 (4-bit)")
+        raise ValueError(f"cache dtype {kind} is neither {dtype} nor uint8 (4-bit)")
     if row != want:
         raise ValueError(f"a cache row must have {want} elements, got {row}")
-    ps, hs, ts, es = k.stride()
-    if es != 1 and row > 1:
+    if es != 1:
         raise ValueError("a cache row must be contiguous")
-    if size < 1 or size & (size - 1) or size > 65536:
+    if heads < 1 or size < 1 or size & (size - 1) or size > 65536:
         raise ValueError(f"page_size must be a power of two up to 65536, got {size}")
-    if (ps * elem) % 16 or (hs * elem) % 16 or (ts * elem) % 16:
+    if (ps | hs | ts) & 15:
         raise ValueError("cache strides must be multiples of 16 bytes")
-    return _native.PagedCache(k.data_ptr(), v.data_ptr(), pages, ps * elem, hs * elem, ts * elem, heads, size,
-                              head_dim, bits)
+    return k.data_ptr(), v.data_ptr(), pages, ps, hs, ts, heads, size, head_dim, bits
 
 
-def _rows(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, dev: torch.device):
-    """Checks [n, heads, head_dim] rows; strides of the first two dimensions are free."""
-    if t.dim() != 3 or t.shape[0] != n:
-        raise ValueError(f"{name} must be [{n}, heads, head_dim]")
-    if t.dtype != dtype or t.device != dev:
+def _rows(name: str, t: torch.Tensor, shape, dtype: torch.dtype, dev: int):
+    """Checks [n, heads, head_dim] rows (the first two strides are free); returns those strides."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if t.dtype != dtype or t.get_device() != dev:
         raise ValueError(f"{name} must have the dtype and device of q")
     ts, hs, es = t.stride()
-    if es != 1 or ts % 8 or hs % 8:
+    if es != 1 or (ts | hs) & 7:
         raise ValueError(f"{name}: head_dim must be contiguous and the other strides multiples of 8")
     return ts, hs
 
 
-def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, n: int, dev: torch.device):
-    if t.dtype != dtype or t.dim() != 1 or t.numel() != n or t.device != dev or not t.is_contiguous():
+def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, n: int, dev: int) -> int:
+    if t.dtype != dtype or t.shape != (n,) or t.get_device() != dev or (n > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} must be contiguous {dtype} [{n}] on the device of q")
     return t.data_ptr()
 
 
-def _call(dev: torch.device, name: str, *args):
-    """The library call on the tensors' device, whichever is current."""
-    if torch.cuda.current_device() == dev.index:
-        return _native.call(name, *args, _stream_ptr(dev))
+def _launch(dev: int, fn, *args):
+    """The library call on the tensors' device, whichever is current, and its current stream."""
+    if torch._C._cuda_getDevice() == dev:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     with torch.cuda.device(dev):
-        return _native.call(name, *args, _stream_ptr(dev))
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev))
 
 
-def _status_word(status: Optional[torch.Tensor], dev: torch.device):
+def _status_word(status: Optional[torch.Tensor], dev: int):
     """(word to pass or None, whether to read it here): the caller's, or one of this call's own when
     ``SMB_DEBUG=1``."""
     if status is not None:
-        if status.dtype != torch.int32 or status.numel() != 1 or status.device != dev:
+        if status.dtype != torch.int32 or status.numel() != 1 or status.get_device() != dev:
             raise ValueError("status must be int32 [1] on the device of q")
         return status, False
     if ops.DEBUG:
-        return torch.zeros(1, dtype=torch.int32, device=dev), True
+        return torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", dev)), True
     return None, False
 
 
@@ -197,8 +197,18 @@ BAD_PAGE = 2
 
 
 def _raise_status(name: str, status: torch.Tensor):
-    if int(status.item()) != 0:
-        _native.check(name + " (device status)", -10 if int(status.item()) == BAD_PAGE else -9)
+    code = int(status.item())
+    if code != 0:
+        _native.check(name + " (device status)", -10 if code == BAD_PAGE else -9)
+
+
+def _query(q: torch.Tensor):
+    if not q.is_cuda:
+        raise ValueError("q must be a CUDA tensor (no host path exists)")
+    shape = q.shape
+    if len(shape) != 3 or shape[1] < 1:
+        raise ValueError("q must be [N, heads, head_dim]")
+    return q.get_device(), q.dtype, ops.storage_code(q.dtype), shape
 
 
 def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -216,38 +226,34 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
     ``interleaved``; both None: no rotation.  ``q_norm`` / ``k_norm`` [head_dim]: weights of an RMS norm
     of each head before the rotation.  ``status`` int32 [1], set to :data:`BAD_PAGE` by a slot past
     the cache (which is not written)."""
-    if not q.is_cuda:
-        raise ValueError("q must be a CUDA tensor (no host path exists)")
-    if q.dim() != 3:
-        raise ValueError("q must be [N, heads, head_dim]")
-    dev, dtype = q.device, q.dtype
-    code = ops.storage_code(dtype)
-    N, Hq, D = q.shape
+    dev, dtype, code, shape = _query(q)
+    N, Hq, D = shape
     cache = _cache(k_cache, v_cache, D, dtype, dev)
-    strides = (ctypes.c_int64 * 6)(*_rows("q", q, N, dtype, dev), *_rows("k", k, N, dtype, dev),
-                                   *_rows("v", v, N, dtype, dev))
-    if k.shape[1:] != (cache.kv_heads, D) or v.shape[1:] != (cache.kv_heads, D):
-        raise ValueError(f"k and v must be [{N}, {cache.kv_heads}, {D}]")
+    kv_shape = (N, cache[6], D)
+    strides = _rows("q", q, shape, dtype, dev) + _rows("k", k, kv_shape, dtype, dev) + _rows("v", v, kv_shape, dtype, dev)
     slots_p = _vector("slots", slots, torch.int64, N, dev)
     rot = pos_p = freq_p = 0
     if (positions is None) != (inv_freq is None):
         raise ValueError("positions and inv_freq go together")
     if inv_freq is not None:
         rot = 2 * inv_freq.numel()
-        if rot % 16 or rot > D:
+        if rot & 15 or rot > D:
             raise ValueError(f"inv_freq must have a multiple of 8 entries, at most {D // 2}")
         pos_p = _vector("positions", positions, torch.int64, N, dev)
         freq_p = _vector("inv_freq", inv_freq, torch.float64, rot // 2, dev)
-    qn_p = None if q_norm is None else _vector("q_norm", q_norm, dtype, D, dev)
-    kn_p = None if k_norm is None else _vector("k_norm", k_norm, dtype, D, dev)
+    qn_p = 0 if q_norm is None else _vector("q_norm", q_norm, dtype, D, dev)
+    kn_p = 0 if k_norm is None else _vector("k_norm", k_norm, dtype, D, dev)
     if out is None:
-        out = torch.empty(N, Hq, D, dtype=dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != dtype or out.device != dev or not out.is_contiguous():
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype != dtype or out.get_device() != dev or not out.is_contiguous():
         raise ValueError("out must be contiguous, with the shape, dtype and device of q")
     word, mine = _status_word(status, dev)
-    _call(dev, "smb_kv_append", ctypes.byref(cache), q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, code, N, Hq,
-          slots_p, pos_p or None, freq_p or None, rot, int(interleaved), float(rope_scale), qn_p, kn_p, float(eps),
-          out.data_ptr(), None if word is None else word.data_ptr())
+    args = _native.APPEND_ARGS
+    rc = _launch(dev, _native.load().smb_kv_append, args.pack(
+        args.size, *cache, q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides, slots_p, pos_p, freq_p, qn_p, kn_p,
+        out.data_ptr(), 0 if word is None else word.data_ptr(), code, N, Hq, rot, bool(interleaved), rope_scale, eps))
+    if rc:
+        _native.check("smb_kv_append", rc)
     if mine:
         _raise_status("smb_kv_append", word)
     return out
@@ -261,17 +267,19 @@ def kv4_read(cache: torch.Tensor, slots: torch.Tensor, head_dim: int, dtype: tor
         raise ValueError("cache must be a CUDA tensor (no host path exists)")
     if cache.dtype != torch.uint8:
         raise ValueError("cache must be a 4-bit cache (uint8)")
-    dev = cache.device
+    dev = cache.get_device()
     code = ops.storage_code(dtype)
     c = _cache(cache, cache, head_dim, dtype, dev)
     M = slots.numel()
     slots_p = _vector("slots", slots, torch.int64, M, dev)
+    shape = (M, c[6], head_dim)
     if out is None:
-        out = torch.empty(M, c.kv_heads, head_dim, dtype=dtype, device=dev)
-    elif out.shape != (M, c.kv_heads, head_dim) or out.dtype != dtype or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous {dtype} [{M}, {c.kv_heads}, {head_dim}] on the cache's device")
-    _call(dev, "smb_kv4_read", cache.data_ptr(), c.num_pages, c.kv_heads, c.page_size, head_dim, c.page_stride,
-          c.head_stride, c.token_stride, code, slots_p, M, out.data_ptr())
+        out = torch.empty(shape, dtype=dtype, device=cache.device)
+    elif out.shape != shape or out.dtype != dtype or out.get_device() != dev or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {dtype} {list(shape)} on the cache's device")
+    rc = _launch(dev, _native.load().smb_kv4_read, _native.CACHE_ARGS.pack(*c), code, slots_p, M, out.data_ptr())
+    if rc:
+        _native.check("smb_kv4_read", rc)
     return out
 
 
@@ -286,69 +294,64 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``block_table`` int32 [B, max_pages], ``kv_lens`` int32 [B], ``q_starts`` int32 [B + 1].  Without
     ``tree`` the new tokens are causal.  ``tree`` int32 [N, words] (:func:`pack_mask`,
     :func:`tree_words`): token i sees every key before the sequence's new tokens, and new token t
-    where bit t is set.  ``scale`` (positive) defaults to
-    head_dim ** -0.5.  ``lse`` float32 [N, Hq], optional:
-    receives the natural log of each softmax's sum (-inf, with an output of 0, for a token that sees no
-    key).  Rows of q behind the last sequence leave ``out`` and ``lse`` as they were.  ``out`` may not
-    overlap q.  ``status`` int32 [1] is set to :data:`BAD_PAGE` by a page outside the cache (its keys
-    are left out)."""
-    if not q.is_cuda:
-        raise ValueError("q must be a CUDA tensor (no host path exists)")
-    if q.dim() != 3:
-        raise ValueError("q must be [N, heads, head_dim]")
-    dev, dtype = q.device, q.dtype
-    code = ops.storage_code(dtype)
-    N, Hq, D = q.shape
+    where bit t is set.  ``scale`` (positive) defaults to head_dim ** -0.5.  ``lse`` float32 [N, Hq],
+    optional: receives the natural log of each softmax's sum (-inf, with an output of 0, for a token
+    that sees no key).  Rows of q behind the last sequence leave ``out`` and ``lse`` as they were.
+    ``out`` may not overlap q.  ``status`` int32 [1] is set to :data:`BAD_PAGE` by a page outside the
+    cache (its keys are left out)."""
+    dev, dtype, code, shape = _query(q)
+    N, Hq, D = shape
     cache = _cache(k_cache, v_cache, D, dtype, dev)
-    qts, qhs = _rows("q", q, N, dtype, dev)
-    if Hq == 0 or Hq % cache.kv_heads:
-        raise ValueError(f"{Hq} query heads are not a multiple of {cache.kv_heads} key heads")
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.device != dev:
+    qts, qhs = _rows("q", q, shape, dtype, dev)
+    if Hq % cache[6]:
+        raise ValueError(f"{Hq} query heads are not a multiple of {cache[6]} key heads")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.get_device() != dev:
         raise ValueError("block_table must be int32 [B, max_pages] on the device of q")
     B, max_pages = block_table.shape
-    if max_pages > 1 and block_table.stride(1) != 1:
+    table_stride, one = block_table.stride()
+    if max_pages > 1 and one != 1:
         raise ValueError("a row of block_table must be contiguous")
     lens_p = _vector("kv_lens", kv_lens, torch.int32, B, dev)
     starts_p = _vector("q_starts", q_starts, torch.int32, B + 1, dev)
-    tree_p, tree_stride, words = None, 0, 0
+    tree_p = tree_stride = words = 0
     if tree is not None:
-        if tree.dim() != 2 or tree.dtype != torch.int32 or tree.shape[0] != N or tree.device != dev:
+        if tree.dim() != 2 or tree.dtype != torch.int32 or tree.shape[0] != N or tree.get_device() != dev:
             raise ValueError("tree must be int32 [N, words] on the device of q")
         words = tree.shape[1]
-        if words < 1 or (words > 1 and tree.stride(1) != 1):
+        tree_stride, one = tree.stride()
+        if words < 1 or (words > 1 and one != 1):
             raise ValueError("tree needs a word for each token, the words contiguous")
-        tree_p, tree_stride = tree.data_ptr(), tree.stride(0)
+        tree_p = tree.data_ptr()
+        if N == 0:
+            tree_p = 0
     if out is None:
-        out = torch.empty(N, Hq, D, dtype=dtype, device=dev)
-    elif out.shape != q.shape:
-        raise ValueError("out must have the shape of q")
-    ots, ohs = _rows("out", out, N, dtype, dev)
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (N, Hq) or lse.device != dev
+        out = q.new_empty(shape)
+    ots, ohs = _rows("out", out, shape, dtype, dev)
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (N, Hq) or lse.get_device() != dev
                             or not lse.is_contiguous()):
         raise ValueError("lse must be contiguous float32 [N, Hq] on the device of q")
-    scale = float(D ** -0.5 if scale is None else scale)
+    scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale <= 1e30:
         raise ValueError(f"scale must be positive and finite, got {scale}")
     word, mine = _status_word(status, dev)
-    nbytes = _workspace_bytes(N, B, Hq, cache, dev)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _call(dev, "smb_paged_attention", ctypes.byref(cache), q.data_ptr(), qts, qhs, code, N, Hq, B,
-          block_table.data_ptr(), block_table.stride(0) if B > 1 else max_pages, max_pages, lens_p, starts_p, tree_p,
-          tree_stride, words, scale, out.data_ptr(), ots, ohs,
-          None if lse is None else lse.data_ptr(), None if word is None else word.data_ptr(), ws.data_ptr(), nbytes)
+    nbytes = _workspace_bytes(N, B, Hq, cache[6], D, cache[9], dev)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    args = _native.ATTENTION_ARGS
+    rc = _launch(dev, _native.load().smb_paged_attention, args.pack(
+        args.size, *cache, q.data_ptr(), qts, qhs, out.data_ptr(), ots, ohs, block_table.data_ptr(), table_stride,
+        lens_p, starts_p, tree_p, tree_stride, 0 if lse is None else lse.data_ptr(),
+        0 if word is None else word.data_ptr(), ws.data_ptr(), nbytes, code, N, Hq, B, max_pages, words, scale))
+    if rc:
+        _native.check("smb_paged_attention", rc)
     if mine:
         _raise_status("smb_paged_attention", word)
     return out
 
 
-def _workspace_bytes(N: int, B: int, Hq: int, cache, dev: torch.device) -> int:
-    fn = _native.load().smb_paged_attention_workspace_bytes
-    if torch.cuda.current_device() == dev.index:
-        n = fn(N, B, Hq, cache.kv_heads, cache.head_dim, cache.bits)
-    else:
-        with torch.cuda.device(dev):
-            n = fn(N, B, Hq, cache.kv_heads, cache.head_dim, cache.bits)
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(N: int, B: int, Hq: int, Hkv: int, D: int, bits: int, dev: int) -> int:
+    with torch.cuda.device(dev):
+        n = _native.load().smb_paged_attention_workspace_bytes(N, B, Hq, Hkv, D, bits)
     if n == 0:
-        raise NotImplementedError(f"unsupported attention sizes N={N} B={B} Hq={Hq} kv_heads={cache.kv_heads} "
-                                  f"head_dim={cache.head_dim}")
+        raise NotImplementedError(f"unsupported attention sizes N={N} B={B} Hq={Hq} kv_heads={Hkv} head_dim={D}")
     return int(n)

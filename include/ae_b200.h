@@ -391,21 +391,30 @@ SMB_API int smb_kv4_row_bytes(int head_dim);
  * (rot a multiple of 16, 0: none; pairs (i, i + rot/2), or (2i, 2i + 1) when `interleaved`;
  * angle = positions[t] * inv_freq[i] in 64 bits, cos and sin times rope_scale), then queries to
  * q_out [N, Hq, head_dim] and keys and values to the rows of slots[t] (specmoe/models/mixtral.py:
- * 118-224 rotates and caches in separate kernels).  strides: host array of six, in elements:
- * token and head stride of q, k and v (multiples of 8; head_dim is contiguous).  A negative slot
- * is not written; a slot past the cache is not written and recorded as SMB_ERR_BAD_PAGE's device
- * code in *status (device int, NULL: not recorded).  The slots of a call have to be distinct. */
-SMB_API int smb_kv_append(const smb_paged_cache_t* cache, const void* q, const void* k, const void* v,
-                          const int64_t* strides, int dtype, int N, int Hq, const int64_t* slots,
-                          const int64_t* positions, const double* inv_freq, int rot, int interleaved,
-                          float rope_scale, const void* q_norm, const void* k_norm, float eps, void* q_out,
-                          int* status, smb_stream_t stream);
+ * 118-224 rotates and caches in separate kernels).  Strides {token, head} in elements, multiples of
+ * 8; head_dim is contiguous.  A negative slot is not written; a slot past the cache is not written
+ * and recorded as 2 in *status (device int, NULL: not recorded).  The slots of a call have to be
+ * distinct. */
+typedef struct smb_append_args {
+  size_t struct_bytes; /* sizeof(smb_append_args_t) */
+  smb_paged_cache_t cache;
+  const void *q, *k, *v;
+  int64_t q_strides[2], k_strides[2], v_strides[2];
+  const int64_t* slots;     /* [N] */
+  const int64_t* positions; /* [N], NULL if rot = 0 */
+  const double* inv_freq;   /* [rot / 2], NULL if rot = 0 */
+  const void *q_norm, *k_norm;
+  void* q_out;
+  int* status;
+  int dtype, N, Hq, rot, interleaved;
+  float rope_scale, eps;
+} smb_append_args_t;
+SMB_API int smb_kv_append(const smb_append_args_t* args, smb_stream_t stream);
 
-/* Rows of one 4-bit array (keys or values) as 16-bit values: out [M, kv_heads, head_dim] of `dtype`
- * for slots [M].  A slot outside the cache reads as zeros. */
-SMB_API int smb_kv4_read(const void* cache, int64_t num_pages, int kv_heads, int page_size, int head_dim,
-                         int64_t page_stride, int64_t head_stride, int64_t token_stride, int dtype,
-                         const int64_t* slots, int M, void* out, smb_stream_t stream);
+/* Rows of the key array (cache.k) of a 4-bit cache as 16-bit values: out [M, kv_heads, head_dim] of
+ * `dtype` for slots [M].  A slot outside the cache reads as zeros.  (Values: pass them as cache.k.) */
+SMB_API int smb_kv4_read(const smb_paged_cache_t* cache, int dtype, const int64_t* slots, int M, void* out,
+                         smb_stream_t stream);
 
 /* Bytes of workspace one smb_paged_attention call needs (0 for invalid sizes).  It needs no
  * initialisation and holds nothing between calls. */
@@ -418,18 +427,32 @@ SMB_API size_t smb_paged_attention_workspace_bytes(int N, int B, int Hq, int Hkv
  * or, given `tree` [N][tree_words] of 32 bits each, if j < P or bit j - P of its words is set (draft
  * trees: ancestors and itself; bits beyond the words read as 0).  out = softmax(scale * q k) v,
  * lse [N, Hq] (optional) = the natural log of the softmax's sum; a token that sees no key gets 0 and
- * -inf.  Rows of q that belong to no sequence leave out and lse as they were.  Lengths are read on the
- * device: kv_lens is cut to max_pages * page_size, q_starts to [0, N]; keys of a page outside
- * [0, num_pages) are left out and recorded in *status (device int, optional).
+ * -inf.  Rows of q that belong to no sequence leave out and lse as they were; out may not overlap q.
+ * Lengths are read on the device: kv_lens is cut to max_pages * page_size, q_starts to [0, N]; keys of
+ * a page outside [0, num_pages) are left out and recorded as 2 in *status (device int, optional).
  * (specmoe/layers/attention_backend/triton_backend.py, cpu_backend.py; the lse is what joins a
  * result with another part of the context, as the reference joins its CPU and GPU parts.) */
-SMB_API int smb_paged_attention(const smb_paged_cache_t* cache, const void* q, int64_t q_token_stride,
-                                int64_t q_head_stride, int dtype, int N, int Hq, int B,
-                                const int32_t* block_table, int64_t table_stride, int max_pages,
-                                const int32_t* kv_lens, const int32_t* q_starts, const int32_t* tree,
-                                int64_t tree_stride, int tree_words, float scale, void* out,
-                                int64_t out_token_stride, int64_t out_head_stride, float* lse, int* status,
-                                void* ws, size_t ws_bytes, smb_stream_t stream);
+typedef struct smb_attention_args {
+  size_t struct_bytes; /* sizeof(smb_attention_args_t) */
+  smb_paged_cache_t cache;
+  const void* q;
+  int64_t q_strides[2]; /* {token, head}, elements, multiples of 8 */
+  void* out;
+  int64_t out_strides[2];
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* kv_lens;  /* [B] */
+  const int32_t* q_starts; /* [B + 1] */
+  const int32_t* tree;     /* NULL: causal */
+  int64_t tree_stride;
+  float* lse;
+  int* status;
+  void* ws;
+  size_t ws_bytes;
+  int dtype, N, Hq, B, max_pages, tree_words;
+  float scale; /* positive */
+} smb_attention_args_t;
+SMB_API int smb_paged_attention(const smb_attention_args_t* args, smb_stream_t stream);
 
 #ifdef __cplusplus
 }
