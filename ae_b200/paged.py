@@ -335,7 +335,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError(f"scale must be positive and finite, got {scale}")
     word, mine = _status_word(status, dev)
     nbytes = _workspace_bytes(N, B, Hq, cache[6], D, cache[9], dev)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    ws = q.new_empty(nbytes >> 1)  # 16-bit elements
     args = _native.ATTENTION_ARGS
     rc = _launch(dev, _native.load().smb_paged_attention, args.pack(
         args.size, *cache, q.data_ptr(), qts, qhs, out.data_ptr(), ots, ohs, block_table.data_ptr(), table_stride,
