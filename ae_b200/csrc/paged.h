@@ -82,6 +82,7 @@ struct AttnArgs {
   float* part_ml;  // [2 * grid][R][2] their running maximum (log2 units) and sum
   JoinRecord* records;  // [grid]
   int min_tiles;        // fewest key tiles worth a CTA of its own
+  int seg_cost;         // what a segment's start and end cost a CTA, in key tiles
 };
 
 cudaError_t launch_kv_append(const AppendArgs& a, int D, bool bf16, bool bits4, int sms, cudaStream_t stream, bool pdl);
@@ -91,6 +92,7 @@ cudaError_t launch_kv4_read(const Kv4ReadArgs& a, int D, bool bf16, cudaStream_t
 struct AttnPlan {
   int rows;  // R: rows of a row tile
   int grid;
+  int min_tiles, seg_cost;
 };
 AttnPlan plan_attn_mma(int N, int B, int g, int D, bool bits4, int sms);
 cudaError_t launch_attn_mma(AttnArgs a, const AttnPlan& p, int D, bool bf16, bool bits4, cudaStream_t stream, bool pdl);

@@ -569,8 +569,10 @@ __global__ void __launch_bounds__(128, (MmaCfg<D, MT, BITS4>::CTAS > 2 && MT == 
         if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * R + r) * 2) = make_float2(top, sum);
       }
     }
-    if (k.w + (t1 - t0) >= k.w_hi && tid == 0) leave_record(a, cta, k);
-    if (!work_next<BK>(a, W, cta, gridDim.x, k)) break;
+    if (k.final || !work_next<BK>(a, W, cta, gridDim.x, k)) {
+      if (tid == 0) leave_record(a, cta, k);
+      break;
+    }
     __syncthreads();  // the merge buffer is the next segment's ring
   }
 }
@@ -663,6 +665,8 @@ AttnPlan plan_attn_mma(int N, int B, int g, int D, bool bits4, int sms) {
   const long long rows = (static_cast<long long>(N) * g + B - 1) / B;
   p.rows = rows > 16 && D <= 128 ? 32 : 16;
   p.grid = sms * by_size<__half>(D, p.rows, bits4).ctas;
+  p.min_tiles = 2;
+  p.seg_cost = 4;
   return p;
 }
 

@@ -25,6 +25,10 @@
 // a mask cuts a tile, the softmax warps look through V in shared memory before the product, take
 // non-finite values out, and the rows that do see them get them added from memory at the end.
 //
+// Q comes by TMA too, one box of tq tokens x gs heads and 64 dims, as soon as the last segment's
+// products with Q are done, so that a segment's first S is there when its predecessor's output has been
+// written.
+//
 // Every wait is bounded, and no role waits at a hardware barrier inside its loop: after a failed wait
 // each role runs out of segments by itself (the results are void, the status says so).
 #include <algorithm>
@@ -48,10 +52,10 @@ template <int D, bool DUAL>
 struct TcCfg {
   static constexpr int R = DUAL ? 256 : 128;
   static constexpr int TILE = kTBK * D * 2;                 // bytes of a K or V tile, and of 128 rows of Q
-  // (the single row tile's place also holds the streams' exchange of outputs: 2 x 32 columns)
-  static constexpr int Q = DUAL ? 2 * TILE : TILE > 32768 ? TILE : 32768;
-  static constexpr int SMEM = Q + kTSlots * TILE + 1024;
-  static_assert(DUAL || Q >= 2 * 128 * 32 * 4, "room for the streams' exchange");
+  static constexpr int QHALF = R * 128;                     // bytes of 64 dims of Q
+  static constexpr int Q = (DUAL ? 2 : 1) * TILE;
+  static constexpr int GIVE = DUAL ? 0 : 2 * 128 * 32 * 4;  // 32 columns of each stream's output for the other
+  static constexpr int SMEM = Q + kTSlots * TILE + GIVE + 1024;
 };
 
 // TMEM columns: S of the streams at 0 and 128 (P in their first 64), O at 256 and 384.
@@ -63,6 +67,14 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
           "r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::
+          "r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
 
@@ -146,20 +158,19 @@ constexpr int kTSegReaders = 1 + 1 + 256;  // TMA and MMA warps, softmax threads
 
 template <int D, bool DUAL, typename T>
 __global__ void __launch_bounds__(kTThreads, 1)
-    paged_attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap tm_k,
-                         const __grid_constant__ CUtensorMap tm_v) {
+    paged_attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap tm_q,
+                         const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   using C = TcCfg<D, DUAL>;
   using H = Half2<T>;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int R = C::R, TILE = C::TILE;
   constexpr uint32_t HALF = kTBK * 128;  // bytes of 64 dims of a tile
   extern __shared__ uint8_t dyn_smem[];
-  __shared__ uint64_t full_bar[kTSlots], empty_bar[kTSlots], s_bar[2], p_bar[2][2], o_bar[2], q_bar[2], drain_bar, both_bar;
+  __shared__ uint64_t full_bar[kTSlots], empty_bar[kTSlots], s_bar[2], p_bar[2][2], o_bar[2], q_full, q_empty, drain_bar, both_bar;
   __shared__ uint64_t seg_full[kTSegs], seg_empty[kTSegs];
   __shared__ Segment s_seg[kTSegs];
   __shared__ uint32_t s_tmem, s_pages[kTOkRing];
   __shared__ int s_abort, s_fix;
-  __shared__ float2 s_ml[2][DUAL ? 1 : 128];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t raw = smem_u32(dyn_smem);
@@ -182,15 +193,17 @@ __global__ void __launch_bounds__(kTThreads, 1)
       mbar_init(&p_bar[i][0], 128);
       mbar_init(&p_bar[i][1], 128);
       mbar_init(&o_bar[i], 1);
-      mbar_init(&q_bar[i], 128);
     }
     for (int i = 0; i < kTSegs; ++i) {
       mbar_init(&seg_full[i], 1);
       mbar_init(&seg_empty[i], kTSegReaders);
     }
+    mbar_init(&q_full, 1);
+    mbar_init(&q_empty, 1);
     mbar_init(&drain_bar, 1);
     mbar_init(&both_bar, 256);
     fence_mbarrier_init();
+    prefetch_tmap(&tm_q);
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
   }
@@ -254,15 +267,22 @@ __global__ void __launch_bounds__(kTThreads, 1)
         };
         while (__all_sync(0xffffffffu, next_segment(seg, g))) {
           if (lane == 0) mbar_arrive(&seg_empty[seg % kTSegs]);
-          ++seg;
           const int n = g.t1 - g.t0;
+          load(&tm_k, g.t0, true);
+          mbar_wait(&q_empty, (seg & 1) ^ 1, status, abort_flag);
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&q_full, a.tq * a.gs * (D / 64) * 128);
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) tma_load_3d(q_s + h * C::QHALF, &tm_q, &q_full, h * 64, g.head, g.tok);
+          }
+          __syncwarp();
+          ++seg;
           if constexpr (DUAL) {
             for (int t = g.t0; t < g.t1; ++t) {
-              load(&tm_k, t, true);
+              if (t > g.t0) load(&tm_k, t, true);
               load(&tm_v, t, false);
             }
           } else {
-            load(&tm_k, g.t0, true);
             if (n > 1) load(&tm_k, g.t0 + 1, true);
             for (int i = 0; i < n; ++i) {
               load(&tm_v, g.t0 + i, false);
@@ -273,11 +293,12 @@ __global__ void __launch_bounds__(kTThreads, 1)
         // the copies into every slot have landed before the CTA may end
         for (int i = max(0, it - kTSlots); i < it; ++i)
           mbar_wait(&full_bar[i % kTSlots], (i / kTSlots) & 1, status, nullptr);
-      } else if (warp == 3 && lane == 0) {
+        if (seg > 0) mbar_wait(&q_full, (seg - 1) & 1, status, nullptr);
+      } else if (warp == 3) {
         // ---------------------------------------------------------------- segments
         Work k;
         bool more = work_begin<kTBK>(a, plan, W, cta, gridDim.x, k);
-        if (!more) leave_record(a, cta, k);
+        if (!more && lane == 0) leave_record(a, cta, k);
         while (more) {
           const Cursor& cur = k.cur;
           Segment n;
@@ -296,15 +317,20 @@ __global__ void __launch_bounds__(kTThreads, 1)
           n.prefix = cur.s.L - cur.s.n;
           n.open = a.tree != nullptr ? n.prefix : n.prefix + n.i0 + 1;
           mbar_wait(&seg_empty[seg % kTSegs], ((seg / kTSegs) & 1) ^ 1, status, abort_flag);
-          s_seg[seg % kTSegs] = n;
-          mbar_arrive(&seg_full[seg % kTSegs]);
+          if (lane == 0) {
+            s_seg[seg % kTSegs] = n;
+            mbar_arrive(&seg_full[seg % kTSegs]);
+          }
+          __syncwarp();
           ++seg;
-          if (k.w + (k.t1 - k.t0) >= k.w_hi) leave_record(a, cta, k);
-          more = work_next<kTBK>(a, W, cta, gridDim.x, k);
+          more = !k.final && work_next<kTBK>(a, W, cta, gridDim.x, k);
+          if (!more && lane == 0) leave_record(a, cta, k);
         }
         mbar_wait(&seg_empty[seg % kTSegs], ((seg / kTSegs) & 1) ^ 1, status, abort_flag);
-        s_seg[seg % kTSegs].t1 = -1;
-        mbar_arrive(&seg_full[seg % kTSegs]);
+        if (lane == 0) {
+          s_seg[seg % kTSegs].t1 = -1;
+          mbar_arrive(&seg_full[seg % kTSegs]);
+        }
       } else if (warp == 1 && lane == 0) {
         // ---------------------------------------------------------------- MMA
         constexpr uint32_t idesc_s = idesc_f16(kBF16, 128, kTBK);
@@ -315,11 +341,11 @@ __global__ void __launch_bounds__(kTThreads, 1)
           tc_fence_after();
         };
         auto qk = [&](int i, int s) {  // S_s = Q_s K^T, K in the slot of step i
-          const uint32_t ks = ring_s + (i % kTSlots) * TILE, qs = q_s + (DUAL ? s * TILE : 0);
+          const uint32_t ks = ring_s + (i % kTSlots) * TILE, qs = q_s + (DUAL ? s * (128 * 128) : 0);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk / 4) * HALF + (kk % 4) * 32;
-            umma_f16(tmem + kTmemS + s * 128, desc_kmajor_sw128(qs + off), desc_kmajor_sw128(ks + off), idesc_s, kk > 0);
+            const uint32_t qo = (kk / 4) * C::QHALF + (kk % 4) * 32, ko = (kk / 4) * HALF + (kk % 4) * 32;
+            umma_f16(tmem + kTmemS + s * 128, desc_kmajor_sw128(qs + qo), desc_kmajor_sw128(ks + ko), idesc_s, kk > 0);
           }
         };
         // O_s (+)= P_s V, each half as soon as its 64 keys of P are there
@@ -339,8 +365,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
         while (next_segment(seg, g)) {
           mbar_arrive(&seg_empty[seg % kTSegs]);
           const int n = g.t1 - g.t0;
-          mbar_wait(&q_bar[0], seg & 1, status, abort_flag);
-          mbar_wait(&q_bar[1], seg & 1, status, abort_flag);
+          mbar_wait(&q_full, seg & 1, status, abort_flag);
           tc_fence_after();
           ++seg;
           if constexpr (DUAL) {
@@ -351,6 +376,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
             qk(kslot, 1);
             umma_commit(&s_bar[1]);
             umma_commit(&empty_bar[kslot % kTSlots]);
+            if (n == 1) umma_commit(&q_empty);
             for (int t = 0; t < n; ++t) {
               const bool more = t + 1 < n;
               const int vslot = it++;
@@ -370,6 +396,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 qk(kslot, 1);
                 umma_commit(&s_bar[1]);
                 umma_commit(&empty_bar[kslot % kTSlots]);
+                if (t + 2 == n) umma_commit(&q_empty);  // the segment's last product with Q
               } else {
                 umma_commit(&o_bar[1]);
               }
@@ -382,6 +409,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
               umma_commit(&s_bar[s]);
               ++it;
             }
+            if (n <= 2) umma_commit(&q_empty);
             for (int t = 0; t < n; ++t) {
               const int s = t & 1;
               wait_full(it);
@@ -393,6 +421,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 qk(it, s);
                 umma_commit(&empty_bar[it % kTSlots]);
                 umma_commit(&s_bar[s]);
+                if (t + 3 == n) umma_commit(&q_empty);  // the segment's last product with Q
                 ++it;
               } else {
                 umma_commit(&o_bar[s]);
@@ -428,26 +457,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
         const bool row_ok = tok_r < g.toks && sub_r < g.heads;
         const long long tok = g.tok + tok_r;
         const int head = g.head + sub_r;
-        // ---- Q: 16-byte chunks of a row, swizzled as TMA would write them
-        {
-          const int rq = DUAL ? r : (tid - 128) & 127;
-          const int tokq = rq / a.gs, subq = rq % a.gs;
-          const bool okq = tokq < g.toks && subq < g.heads;
-          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (g.tok + tokq) * a.q_ts +
-                                                            (g.head + subq) * a.q_hs);
-          constexpr int CH = D / 8;
-          const int c0 = DUAL ? 0 : s * (CH / 2), c1 = DUAL ? CH : c0 + CH / 2;
-          const int rr = rq & 127;
-          uint8_t* dst = sm + (DUAL ? s * TILE : 0) + rr * 128;
-#pragma unroll
-          for (int c = 0; c < CH; ++c) {
-            if (c < c0 || c >= c1) continue;
-            const uint4 v = okq ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(dst + (c >> 3) * HALF + (((c & 7) ^ (rr & 7)) << 4)) = v;
-          }
-          fence_async_proxy();
-          mbar_arrive(&q_bar[s]);
-        }
+        const bool some = __any_sync(0xffffffffu, row_ok);  // a row of this warp is in use
         float m = kNegInf, l = 0.f;
         auto visible = [&](int j) {  // this row, key j
           if (!row_ok || j >= g.keys) return false;
@@ -464,13 +474,12 @@ __global__ void __launch_bounds__(kTThreads, 1)
             // V: what no mask stops from entering the product has to be finite
             const int vstep = it + (DUAL ? 2 * i + 1 : i + min(i + 2, n));
             mbar_wait(&full_bar[vstep % kTSlots], (vstep / kTSlots) & 1, status, abort_flag);
-            uint8_t* vp = sm + C::Q + (vstep % kTSlots) * TILE + row * 128;
-            const bool dead = j0 + row >= g.keys;  // a row behind the keys
+            uint4* vp = reinterpret_cast<uint4*>(sm + C::Q + (vstep % kTSlots) * TILE);
             bool bad = false;
 #pragma unroll 4
             for (int c = 0; c < D / 8; ++c) {
-              uint4* p = reinterpret_cast<uint4*>(vp + (c >> 3) * HALF + ((c & 7) << 4));
-              uint4 v = *p;
+              const int at = c * 128 + (tid & 127);  // 16 bytes of key (at / 8) % 128
+              uint4 v = vp[at];
               uint32_t* u = reinterpret_cast<uint32_t*>(&v);
               bool hit = false;
 #pragma unroll
@@ -480,15 +489,22 @@ __global__ void __launch_bounds__(kTThreads, 1)
               }
               if (hit) {
                 bad = true;
-                if (!dead) *reinterpret_cast<volatile int*>(&s_fix) = 1;  // before the value goes
+                // (not for rows behind the keys; before the value goes)
+                if (j0 + ((at >> 3) & 127) < g.keys) *reinterpret_cast<volatile int*>(&s_fix) = 1;
                 __threadfence_block();
-                *p = v;
+                vp[at] = v;
               }
             }
             if (bad) fence_async_proxy();
           }
           mbar_wait(&s_bar[s], ns & 1, status, abort_flag);
           tc_fence_after();
+          if (!some) {  // nothing to weigh: the product may have what is there
+            mbar_arrive(&p_bar[s][0]);
+            mbar_arrive(&p_bar[s][1]);
+            ++ns;
+            continue;
+          }
           const uint32_t pages_ok = s_pages[(tc + i) % kTOkRing];
           const bool masked = cut || pages_ok != 0xffffffffu;
           uint32_t x[4][32];
@@ -533,7 +549,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; e += 2)
               top[(e >> 1) & 3] = max3(top[(e >> 1) & 3], __uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1]));
-          const float tmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+          const float tmax = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
           // a row is rescaled only when its maximum grew by more than 8 (p stays below 2^8)
           const bool grew = tmax > m + 8.f;
           if (__any_sync(0xffffffffu, grew)) {
@@ -593,9 +609,11 @@ __global__ void __launch_bounds__(kTThreads, 1)
         const long long slot = g.slot;
         float f_own = 1.f, f_other = 0.f;
         if constexpr (!DUAL) {
-          s_ml[s][row] = make_float2(m, l);
+          float2* ml = reinterpret_cast<float2*>(sm + C::Q + kTSlots * TILE);
+          ml[s * 128 + row] = make_float2(m, l);
           both();
-          const float2 o = s_ml[s ^ 1][row];
+          const float2 o = ml[(s ^ 1) * 128 + row];
+          both();  // (the outputs go to the same place)
           const float mx = fmaxf(m, o.x);
           // a stream with no visible key has a maximum of -inf and an output of 0
           f_own = m == kNegInf ? 1.f : exp2_fast(m - mx);
@@ -663,11 +681,10 @@ __global__ void __launch_bounds__(kTThreads, 1)
             store_o(q, o);
           }
         } else {
-          // each stream finishes half of the columns: it leaves 32 of the other's columns at a time where Q
-          // was (every product with Q is complete), [column][row]
+          // each stream finishes half of the columns: it leaves the other's, 32 at a time, as [column][row]
           constexpr int HQ = D / 64;
-          float* give = reinterpret_cast<float*>(sm) + s * (32 * 128);
-          const float* take = reinterpret_cast<const float*>(sm) + (s ^ 1) * (32 * 128);
+          float* give = reinterpret_cast<float*>(sm + C::Q + kTSlots * TILE) + s * (32 * 128);
+          const float* take = reinterpret_cast<const float*>(sm + C::Q + kTSlots * TILE) + (s ^ 1) * (32 * 128);
 #pragma unroll 1
           for (int q = 0; q < HQ; ++q) {
             uint32_t o[32];
@@ -696,7 +713,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
         tc_fence_before();
         it += 2 * n;
         tc += n;
-        if constexpr (!DUAL) both();  // both streams are done with Q's place and (m, l)
+        if constexpr (!DUAL) both();  // both streams are done with the exchange
       }
     }
   }
@@ -715,29 +732,42 @@ const void* tc_fn(bool bf16) {
 
 std::atomic<int> g_smem_seen[8][64];
 
-// Rows [page_size][kv_heads][num_pages] of D 16-bit values; boxes of 64 dims x one page's rows.
-bool encode_cache(CUtensorMap* map, const PagedCacheArgs& c, const void* base, int D, bool bf16) {
+bool encode(CUtensorMap* map, const void* base, bool bf16, int rank, const cuuint64_t* dims, cuuint64_t* strides,
+            const cuuint32_t* box) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return false;
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  // (the stride of a dimension of size 1 means nothing; the encoder wants a usable one)
+  for (int i = 1; i < rank; ++i)
+    if (dims[i] == 1) strides[i - 1] = 16;
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base),
+            dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Rows [page_size][kv_heads][num_pages] of D values; boxes of 64 dims x one page's rows (at most a tile).
+bool encode_cache(CUtensorMap* map, const PagedCacheArgs& c, const void* base, int D, bool bf16) {
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), 1ull << c.page_shift, static_cast<cuuint64_t>(c.Hkv),
                               static_cast<cuuint64_t>(c.num_pages)};
-  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(c.token_stride), static_cast<cuuint64_t>(c.head_stride),
-                                 static_cast<cuuint64_t>(c.page_stride)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(c.token_stride), static_cast<cuuint64_t>(c.head_stride),
+                           static_cast<cuuint64_t>(c.page_stride)};
   const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(std::min(1 << c.page_shift, kTBK)), 1, 1};
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
-            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode(map, base, bf16, 4, dims, strides, box);
+}
+
+// Rows [heads][tokens] of q; boxes of 64 dims x gs heads x tq tokens: the rows of a row tile.
+bool encode_queries(CUtensorMap* map, const AttnArgs& a, int D, bool bf16) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(a.c.Hkv) * a.g,
+                              static_cast<cuuint64_t>(a.N)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(a.q_hs) * 2, static_cast<cuuint64_t>(a.q_ts) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.gs), static_cast<cuuint32_t>(a.tq)};
+  return encode(map, a.q, bf16, 3, dims, strides, box);
 }
 
 }  // namespace
 
 bool tc_takes(const PagedCacheArgs& c) {
-  // (strides of dimensions of size 1 mean nothing, but the encoder wants usable ones)
-  const long long most = 1ll << 40;
-  return c.page_shift >= 3 && c.num_pages >= 1 && c.num_pages < 0x7fffffffll && c.token_stride >= 16 &&
-         c.token_stride < most && c.head_stride >= 16 && c.head_stride < most && c.page_stride >= 16 &&
-         c.page_stride < most;
+  return c.page_shift >= 3 && c.num_pages >= 1 && c.num_pages < 0x7fffffffll;
 }
 
 bool plan_attn_tc(int N, int B, int g, int D, bool bits4, int sms, AttnPlan* p) {
@@ -746,12 +776,14 @@ bool plan_attn_tc(int N, int B, int g, int D, bool bits4, int sms, AttnPlan* p) 
   if (rows <= kTcMinRows) return false;
   p->rows = rows > 128 ? 256 : 128;
   p->grid = sms;
+  p->min_tiles = 2;
+  p->seg_cost = 3;
   return true;
 }
 
 cudaError_t launch_attn_tc(AttnArgs a, const AttnPlan& p, int D, bool bf16, cudaStream_t stream, bool pdl, bool* fits) {
-  CUtensorMap tk, tv;
-  *fits = encode_cache(&tk, a.c, a.c.k, D, bf16) && encode_cache(&tv, a.c, a.c.v, D, bf16);
+  CUtensorMap tq, tk, tv;
+  *fits = encode_queries(&tq, a, D, bf16) && encode_cache(&tk, a.c, a.c.k, D, bf16) && encode_cache(&tv, a.c, a.c.v, D, bf16);
   if (!*fits) return cudaSuccess;
   const bool dual = p.rows == 256;
   const void* fn = D == 64 ? (dual ? tc_fn<64, true>(bf16) : tc_fn<64, false>(bf16))
@@ -770,7 +802,7 @@ cudaError_t launch_attn_tc(AttnArgs a, const AttnPlan& p, int D, bool bf16, cuda
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
-  void* params[] = {&a, &tk, &tv};
+  void* params[] = {&a, &tq, &tk, &tv};
   err = cudaLaunchKernelExC(&cfg, fn, params);
   if (err != cudaSuccess) return err;
   return launch_attn_join(a, p, D, bf16, stream, pdl);

@@ -208,7 +208,8 @@ int smb_paged_attention(const smb_attention_args_t* r, smb_stream_t stream) {
     a.part_o = static_cast<float*>(r->ws);
     a.part_ml = a.part_o + static_cast<size_t>(2) * p.grid * p.rows * D;
     a.records = reinterpret_cast<JoinRecord*>(a.part_ml + static_cast<size_t>(4) * p.grid * p.rows);
-    a.min_tiles = 2;
+    a.min_tiles = p.min_tiles;
+    a.seg_cost = p.seg_cost;
     return r->ws_bytes >= attn_ws(p, D);
   };
   if (tc_takes(a.c) && plan_attn_tc(N, B, a.g, D, bits4, di.sms, &p)) {

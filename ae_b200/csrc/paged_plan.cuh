@@ -8,9 +8,9 @@
 //    length, one CTA each, with T the least number of tiles for which the pieces fit the grid (and no
 //    less than min_tiles: a shorter piece costs more in its start and its join than it saves).  A CTA
 //    has one segment to start and to finish, which is what a short call spends its time on.
-//  - the line, where T would exceed an even share by more than a few tiles: the tiles of all segments
-//    in the order (b, vh, qt, tile) form a line of W tiles, of which CTA c takes the c-th part; the
-//    parts' lengths differ by one tile.
+//  - the line, where T would exceed an even share by more than a few tiles: the segments in the order
+//    (b, vh, qt) form a line, each seg_cost units for its start and its end and one unit for each tile,
+//    of which CTA c takes the c-th part; the parts' lengths differ by one unit.
 // A segment that one CTA has to itself is finished there.  One that is cut leaves a partial result in
 // at most two slots per CTA (2c, and on the line 2c + 1 for the segment a share ends in), and a
 // second kernel joins the parts in the order of their CTAs, so the result does not depend on timing.
@@ -56,7 +56,7 @@ __device__ __forceinline__ int tiles_of(int keys) {
   return max(1, keys / BK + (keys % BK != 0));
 }
 
-// a / b, in 32 bits where both fit (a 64-bit division takes some 100 instructions).
+// a / b for a >= 0, b > 0, in 32 bits where both fit (a 64-bit division takes some 100 instructions).
 __device__ __forceinline__ long long quotient(long long a, long long b) {
   if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
   return a / b;
@@ -67,13 +67,14 @@ template <int BK>
 __device__ __forceinline__ long long floor_sum(long long n, long long step, long long b) {
   long long sum = 0, m = BK, a = step;
   while (n > 0) {
-    sum += (n - 1) * n / 2 * (a / m) + n * (b / m);
-    a %= m;
-    b %= m;
+    const long long qa = quotient(a, m), qb = quotient(b, m);
+    sum += (n - 1) * n / 2 * qa + n * qb;
+    a -= qa * m;
+    b -= qb * m;
     const long long y = a * n + b;
     if (y < m) break;
-    n = y / m;
-    b = y % m;
+    n = quotient(y, m);
+    b = y - n * m;
     const long long t = m;
     m = a;
     a = t;
@@ -81,17 +82,17 @@ __device__ __forceinline__ long long floor_sum(long long n, long long step, long
   return sum;
 }
 
-// Tiles of row tiles [0, qt) of one (sequence, vh).
+// Units of row tiles [0, qt) of one (sequence, vh).
 template <int BK>
-__device__ __forceinline__ long long tiles_before(const AttnArgs& a, const Seq& s, int qt) {
+__device__ __forceinline__ long long units_before(const AttnArgs& a, const Seq& s, int qt) {
   if (qt <= 0) return 0;
-  if (s.n <= a.tq) return tiles_of<BK>(keys_of_tile(a, s, 0));
-  if (a.tree != nullptr) return static_cast<long long>(qt) * tiles_of<BK>(s.L);
+  if (s.n <= a.tq) return tiles_of<BK>(keys_of_tile(a, s, 0)) + a.seg_cost;
+  if (a.tree != nullptr) return static_cast<long long>(qt) * (tiles_of<BK>(s.L) + a.seg_cost);
   const int all = row_tiles(a, s);
-  long long sum = 0;
+  long long sum = static_cast<long long>(qt) * a.seg_cost;
   int whole = qt;
   if (qt == all) {  // the last row tile may be short
-    sum = tiles_of<BK>(keys_of_tile(a, s, all - 1));
+    sum += tiles_of<BK>(keys_of_tile(a, s, all - 1));
     whole = all - 1;
   }
   // row tile i ends at key base + (i + 1) tq; those that end at or before key 0 still take a tile
@@ -106,7 +107,7 @@ __device__ __forceinline__ long long tiles_before(const AttnArgs& a, const Seq& 
 
 // Sums over the sequences before each of kPlanThreads runs of consecutive sequences.
 struct PlanShared {
-  long long before[kPlanThreads + 1];  // tiles (line) or pieces
+  long long before[kPlanThreads + 1];  // units (line) or pieces
   long long warp_sum[kPlanThreads / 32];
   Seq seq[kPlanThreads];               // one run, one sequence: up to kPlanThreads sequences
   int fit[kPlanThreads / 32][4];
@@ -116,14 +117,13 @@ struct PlanShared {
 struct Cursor {
   int b, vh, qt;         // segment
   int keys, tiles;       // of the segment
-  int tile;              // current tile inside it
-  long long start;       // first tile of the segment on the line
+  long long start;       // first unit of the segment on the line
   Seq s;
 };
 
 template <int BK>
-__device__ __forceinline__ long long seq_tiles(const AttnArgs& a, const Seq& s) {
-  return tiles_before<BK>(a, s, row_tiles(a, s)) * (a.c.Hkv * a.nsub);
+__device__ __forceinline__ long long seq_units(const AttnArgs& a, const Seq& s) {
+  return units_before<BK>(a, s, row_tiles(a, s)) * (a.c.Hkv * a.nsub);
 }
 
 // Exclusive prefix sums of v over the first kPlanThreads threads into sh->before; every thread calls.
@@ -156,7 +156,7 @@ __device__ __forceinline__ int piece_length(const AttnArgs& a, long long even, i
 }
 __device__ __forceinline__ int pieces_of(int tiles, int T) { return (tiles + T - 1) / T; }
 
-// Every thread of the CTA calls it; the first kPlanThreads do the work.  Returns the tiles W of the
+// Every thread of the CTA calls it; the first kPlanThreads do the work.  Returns the units W of the
 // line.
 template <int BK>
 __device__ long long plan_build(const AttnArgs& a, PlanShared* sh, int grid) {
@@ -168,7 +168,7 @@ __device__ long long plan_build(const AttnArgs& a, PlanShared* sh, int grid) {
   if (t < kPlanThreads) {
     for (int b = t * per; b < min(a.B, (t + 1) * per); ++b) {
       s = seq_at(a, b);
-      v += seq_tiles<BK>(a, s);
+      v += seq_units<BK>(a, s);
       single = single && s.n <= a.tq;
     }
     sh->seq[t] = s;
@@ -217,7 +217,7 @@ __device__ __forceinline__ int plan_run(const PlanShared* sh, long long w) {
   return lo;
 }
 
-// Position of tile w of the line (0 <= w < W).
+// The segment that holds unit w of the line (0 <= w < W).  Called by whole warps, with the same w.
 template <int BK>
 __device__ Cursor plan_locate(const AttnArgs& a, const PlanShared* sh, long long w) {
   const int per = (a.B + kPlanThreads - 1) / kPlanThreads;
@@ -227,35 +227,35 @@ __device__ Cursor plan_locate(const AttnArgs& a, const PlanShared* sh, long long
   c.b = run * per;
   c.s = per == 1 ? sh->seq[run] : seq_at(a, c.b);
   for (int i = 1; i < per && c.b + 1 < a.B; ++i) {  // w < W, so a sequence that holds it comes before B
-    const long long here = seq_tiles<BK>(a, c.s);
+    const long long here = seq_units<BK>(a, c.s);
     if (w < at + here) break;
     at += here;
     ++c.b;
     c.s = seq_at(a, c.b);
   }
   const int qts = row_tiles(a, c.s);
-  const long long per_head = max(1ll, tiles_before<BK>(a, c.s, qts));
+  const long long per_head = max(1ll, units_before<BK>(a, c.s, qts));
   c.vh = static_cast<int>(quotient(w - at, per_head));
   at += c.vh * per_head;
-  int l = 0, h = qts;
-  while (h - l > 1) {
-    const int mid = (l + h) / 2;
-    if (at + tiles_before<BK>(a, c.s, mid) <= w) l = mid;
-    else h = mid;
+  int l = 0, h = qts;  // the last row tile that begins at or before w is in [l, h)
+  while (h - l > 1) {  // a lane a candidate
+    const int step = (h - l + 31) / 32, mine = l + static_cast<int>(threadIdx.x & 31) * step;
+    const bool before = mine < h && at + units_before<BK>(a, c.s, mine) <= w;
+    const int k = __popc(__ballot_sync(0xffffffffu, before)) - 1;
+    l += k * step;
+    h = min(h, l + step);
   }
   c.qt = l;
-  c.start = at + tiles_before<BK>(a, c.s, l);
+  c.start = at + units_before<BK>(a, c.s, l);
   c.keys = keys_of_tile(a, c.s, l);
   c.tiles = tiles_of<BK>(c.keys);
-  c.tile = static_cast<int>(w - c.start);
   return c;
 }
 
 // The segment after c's (only called while one exists).
 template <int BK>
 __device__ __forceinline__ void plan_next(const AttnArgs& a, Cursor& c) {
-  c.start += c.tiles;
-  c.tile = 0;
+  c.start += c.tiles + a.seg_cost;
   if (++c.qt >= row_tiles(a, c.s)) {
     c.qt = 0;
     if (++c.vh >= a.c.Hkv * a.nsub) {
@@ -270,7 +270,7 @@ __device__ __forceinline__ void plan_next(const AttnArgs& a, Cursor& c) {
   c.tiles = tiles_of<BK>(c.keys);
 }
 
-// The line's shares: CTA c of `ctas` takes [begin(c), begin(c + 1)), the first `more` one tile more
+// The line's shares: CTA c of `ctas` takes [begin(c), begin(c + 1)), the first `more` one unit more
 // than the others.  No share is below min_tiles while that leaves CTAs idle.
 struct Shares {
   long long each;
@@ -293,15 +293,30 @@ struct Work {
   int t0, t1;     // key tiles of the segment that are this CTA's
   int slot;       // where its partial result goes, -1: the segment is this CTA's alone
   int last;       // last CTA with a part of it, if this one has the first of several; -1 otherwise
-  long long w, w_lo, w_hi;
+  bool final;     // no other segment follows
+  long long w, w_hi;
 };
 
-__device__ __forceinline__ void work_open(const Shares& sh, int cta, Work& k) {
-  k.t0 = k.cur.tile;
-  k.t1 = static_cast<int>(min(static_cast<long long>(k.cur.tiles), k.t0 + (k.w_hi - k.w)));
-  const bool whole = k.t0 == 0 && k.t1 == k.cur.tiles;
-  k.slot = whole ? -1 : 2 * cta + (k.cur.start > k.w_lo ? 1 : 0);
-  k.last = k.t0 == 0 && !whole ? sh.owner(k.cur.start + k.cur.tiles - 1) : -1;
+// Opens the next segment of the share [k.w, k.w_hi) of which a tile is in it, k.cur being the one that
+// holds unit k.w; false if there is none.
+template <int BK>
+__device__ __forceinline__ bool work_open(const AttnArgs& a, const Shares& sh, int cta, Work& k) {
+  while (k.w < k.w_hi) {
+    const long long first = k.cur.start + a.seg_cost, end = first + k.cur.tiles;
+    k.t0 = static_cast<int>(max(k.w - first, 0ll));
+    k.t1 = static_cast<int>(min(k.w_hi, end) - first);
+    k.w = end;
+    k.final = end >= k.w_hi;
+    if (k.t1 > k.t0) {
+      const bool whole = k.t0 == 0 && k.t1 == k.cur.tiles;
+      k.slot = whole ? -1 : 2 * cta + (k.t0 == 0);
+      k.last = k.t0 == 0 && !whole ? sh.owner(end - 1) : -1;
+      return true;
+    }
+    if (!k.final) plan_next<BK>(a, k.cur);
+  }
+  k.last = -1;
+  return false;
 }
 
 // This CTA's first segment; false if it has none.
@@ -322,30 +337,26 @@ __device__ bool work_begin(const AttnArgs& a, const PlanShared* sh, long long W,
     k.t1 = k.t0 + len + (p < more);
     k.slot = pieces == 1 ? -1 : 2 * cta;
     if (p == 0 && pieces > 1) k.last = cta + pieces - 1;
-    k.w = k.w_hi = 0;
+    k.final = true;
     return true;
   }
   const Shares line(a, W, grid);
   if (W == 0 || cta >= line.ctas) return false;
-  k.w_lo = line.begin(cta);
+  k.w = line.begin(cta);
   k.w_hi = line.begin(cta + 1);
-  k.w = k.w_lo;
   k.cur = plan_locate<BK>(a, sh, k.w);
-  work_open(line, cta, k);
-  return true;
+  return work_open<BK>(a, line, cta, k);
 }
 
+// The next one (only called after one that is not final).
 template <int BK>
 __device__ __forceinline__ bool work_next(const AttnArgs& a, long long W, int cta, int grid, Work& k) {
-  k.w += k.t1 - k.t0;
-  if (k.w >= k.w_hi) return false;
   plan_next<BK>(a, k.cur);
-  work_open(Shares(a, W, grid), cta, k);
-  return true;
+  return work_open<BK>(a, Shares(a, W, grid), cta, k);
 }
 
-// Notes for the join: called by one thread for the CTA's last segment (the only one that others may
-// go on with), or with none.
+// Notes for the join, by one thread: k.last and the segment it belongs to (the CTA's last one), or
+// that there is none.
 __device__ __forceinline__ void leave_record(const AttnArgs& a, int cta, const Work& k) {
   JoinRecord r;
   r.last = k.last;
