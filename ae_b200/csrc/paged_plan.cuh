@@ -66,6 +66,23 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
 template <int BK>
 __device__ __forceinline__ long long floor_sum(long long n, long long step, long long b) {
   long long sum = 0, m = BK, a = step;
+  if (n < 65536 && step < 65536 && b < 0x7fffffff) {  // (then everything but the sum is below 2^32)
+    unsigned un = static_cast<unsigned>(n), ua = static_cast<unsigned>(step), ub = static_cast<unsigned>(b), um = BK;
+    while (un > 0) {
+      const unsigned qa = ua / um, qb = ub / um;
+      sum += static_cast<long long>(un * (un - 1) / 2) * qa + static_cast<long long>(un) * qb;
+      ua -= qa * um;
+      ub -= qb * um;
+      const unsigned y = ua * un + ub;
+      if (y < um) break;
+      un = y / um;
+      ub = y - un * um;
+      const unsigned t = um;
+      um = ua;
+      ua = t;
+    }
+    return sum;
+  }
   while (n > 0) {
     const long long qa = quotient(a, m), qb = quotient(b, m);
     sum += (n - 1) * n / 2 * qa + n * qb;
