@@ -96,13 +96,14 @@ struct AttnPlan {
 };
 AttnPlan plan_attn_mma(int N, int B, int g, int D, bool bits4, int sms);
 cudaError_t launch_attn_mma(AttnArgs a, const AttnPlan& p, int D, bool bf16, bool bits4, cudaStream_t stream, bool pdl);
-// tcgen05 kernel: false where it does not apply (4-bit caches, heads of 256, pages below 8 tokens, few
-// rows).  launch_attn_tc leaves *fits false, and launches nothing, when the cache's strides do not
+// tcgen05 kernel: plan_attn_tc is false for few rows and heads of 256, tc_takes for 16-bit caches with
+// pages below 8 tokens.  launch_attn_tc leaves *fits false, and launches nothing, when strides do not
 // make a tensor map.
 constexpr int kTcMinRows = 32;  // query rows of a key head, on average over the sequences
-bool tc_takes(const PagedCacheArgs& c);
-bool plan_attn_tc(int N, int B, int g, int D, bool bits4, int sms, AttnPlan* p);
-cudaError_t launch_attn_tc(AttnArgs a, const AttnPlan& p, int D, bool bf16, cudaStream_t stream, bool pdl, bool* fits);
+bool tc_takes(const PagedCacheArgs& c, bool bits4);
+bool plan_attn_tc(int N, int B, int g, int D, int sms, AttnPlan* p);
+cudaError_t launch_attn_tc(AttnArgs a, const AttnPlan& p, int D, bool bf16, bool bits4, cudaStream_t stream, bool pdl,
+                           bool* fits);
 // joins the partial results of the segments that were split over CTAs
 cudaError_t launch_attn_join(const AttnArgs& a, const AttnPlan& p, int D, bool bf16, cudaStream_t stream, bool pdl);
 

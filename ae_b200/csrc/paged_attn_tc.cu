@@ -1,5 +1,5 @@
-// Attention of many query rows over a paged 16-bit cache on the 5th-generation tensor cores:
-// draft trees (a few dozen tokens x the query heads of a key head) and prefill chunks.
+// Attention of many query rows over a paged cache on the 5th-generation tensor cores: draft trees (a
+// few dozen tokens x the query heads of a key head) and prefill chunks.
 //
 //   S = Q K^T  (128 rows x 128 keys, fp32 in TMEM),  P = 2^(scale log2(e) S - m),  O += P V
 //
@@ -29,6 +29,14 @@
 // products with Q are done, so that a segment's first S is there when its predecessor's output has been
 // written.
 //
+// A 4-bit cache has four more warps in the place of TMA's K and V: rows come packed by cp.async into a
+// ring of each warp's own, and go as values of the 16-bit type into the slots (scale x code + zero,
+// one rounding: the score of a key is then off by at most half a step of each of its values, as if the
+// cache were of the 16-bit type; applying the scales to the products instead, as the kernel for few
+// rows does, would need the scores of each group of 32 dims by themselves).  V keeps the order in which
+// a word's nibbles come out (dims e and e + 4 side by side), and the output's columns are put right
+// when they are stored.
+//
 // Every wait is bounded, and no role waits at a hardware barrier inside its loop: after a failed wait
 // each role runs out of segments by itself (the results are void, the status says so).
 #include <algorithm>
@@ -44,18 +52,24 @@ namespace smb {
 namespace {
 
 constexpr int kTBK = 128;       // keys of a tile
-constexpr int kTSlots = 5;      // ring slots
-constexpr int kTThreads = 384;  // warp 0 TMA, warp 1 MMA, warp 2 TMEM, warp 3 segments, warps 4-7 / 8-11 softmax
+// warp 0 TMA, warp 1 MMA, warp 2 TMEM, warp 3 segments, warps 4-7 / 8-11 softmax, 12-15 values of a 4-bit cache
+constexpr int kTThreads = 384, kTThreads4 = 512;
+constexpr int kTRaw = 4;        // slots of packed rows
 constexpr int kTOkRing = 8;     // tiles whose page masks are kept: the ring lets K run at most 5 tiles ahead
 
-template <int D, bool DUAL>
+template <int D, bool DUAL, bool BITS4>
 struct TcCfg {
+  static constexpr int THREADS = BITS4 ? kTThreads4 : kTThreads;
+  static constexpr int NS = BITS4 ? 3 : 5;                  // ring slots
+  static constexpr int ROW4 = kv4_row_bytes(D);
+  static constexpr int RAW = BITS4 ? 4 * kTRaw * 32 * ROW4 : 0;
+  static constexpr int SEG_READERS = 1 + 1 + 256 + (BITS4 ? 128 : 0);  // TMA and MMA warps, softmax threads, ...
   static constexpr int R = DUAL ? 256 : 128;
   static constexpr int TILE = kTBK * D * 2;                 // bytes of a K or V tile, and of 128 rows of Q
   static constexpr int QHALF = R * 128;                     // bytes of 64 dims of Q
   static constexpr int Q = (DUAL ? 2 : 1) * TILE;
   static constexpr int GIVE = DUAL ? 0 : 2 * 128 * 32 * 4;  // 32 columns of each stream's output for the other
-  static constexpr int SMEM = Q + kTSlots * TILE + GIVE + 1024;
+  static constexpr int SMEM = Q + NS * TILE + GIVE + RAW + 1024;
 };
 
 // TMEM columns: S of the streams at 0 and 128 (P in their first 64), O at 256 and 384.
@@ -153,23 +167,41 @@ struct Segment {
   int tok, toks, i0;  // first row of q, tokens, the first one's place among the sequence's new tokens
   int slot;           // of a partial result, -1: the segment lies in this share
 };
-constexpr int kTSegs = 4;                  // segments handed out ahead
-constexpr int kTSegReaders = 1 + 1 + 256;  // TMA and MMA warps, softmax threads
+constexpr int kTSegs = 4;  // segments handed out ahead
 
-template <int D, bool DUAL, typename T>
-__global__ void __launch_bounds__(kTThreads, 1)
+// The k-th of the 2 n loads of a segment of n tiles, in the order of their use.
+template <bool DUAL>
+__device__ __forceinline__ void load_step(int n, int k, int& tile, bool& is_k) {
+  if (DUAL || n == 1) {
+    tile = k >> 1;
+    is_k = (k & 1) == 0;
+  } else if (k < 2) {
+    tile = k;
+    is_k = true;
+  } else {
+    const int j = k - 2, pairs = n - 2;  // (V i, K i + 2) for i < n - 2, then the last two of V
+    is_k = j < 2 * pairs && (j & 1) != 0;
+    tile = j < 2 * pairs ? (is_k ? (j >> 1) + 2 : j >> 1) : j - pairs;
+  }
+}
+
+// Where dim d of a word's eight is among the values that its nibbles give in turn.
+__host__ __device__ constexpr int nibble_place(int d) { return 2 * (d & 3) + (d >> 2); }
+
+template <int D, bool DUAL, bool BITS4, typename T>
+__global__ void __launch_bounds__(BITS4 ? kTThreads4 : kTThreads, 1)
     paged_attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap tm_q,
                          const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
-  using C = TcCfg<D, DUAL>;
+  using C = TcCfg<D, DUAL, BITS4>;
   using H = Half2<T>;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr int R = C::R, TILE = C::TILE;
+  constexpr int R = C::R, TILE = C::TILE, NS = C::NS;
   constexpr uint32_t HALF = kTBK * 128;  // bytes of 64 dims of a tile
   extern __shared__ uint8_t dyn_smem[];
-  __shared__ uint64_t full_bar[kTSlots], empty_bar[kTSlots], s_bar[2], p_bar[2][2], o_bar[2], q_full, q_empty, drain_bar, both_bar;
+  __shared__ uint64_t full_bar[NS], empty_bar[NS], s_bar[2], p_bar[2][2], o_bar[2], q_full, q_empty, drain_bar, both_bar;
   __shared__ uint64_t seg_full[kTSegs], seg_empty[kTSegs];
   __shared__ Segment s_seg[kTSegs];
-  __shared__ uint32_t s_tmem, s_pages[kTOkRing];
+  __shared__ uint32_t s_tmem, s_pages[kTOkRing][BITS4 ? 4 : 1];
   __shared__ int s_abort, s_fix;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -184,8 +216,8 @@ __global__ void __launch_bounds__(kTThreads, 1)
   if (tid == 0) {
     s_abort = 0;
     s_fix = 0;
-    for (int i = 0; i < kTSlots; ++i) {
-      mbar_init(&full_bar[i], 1);
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full_bar[i], BITS4 ? 128 : 1);
       mbar_init(&empty_bar[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -196,7 +228,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
     }
     for (int i = 0; i < kTSegs; ++i) {
       mbar_init(&seg_full[i], 1);
-      mbar_init(&seg_empty[i], kTSegReaders);
+      mbar_init(&seg_empty[i], C::SEG_READERS);
     }
     mbar_init(&q_full, 1);
     mbar_init(&q_empty, 1);
@@ -233,7 +265,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
     Segment g{};
     int seg = 0;
     if (warp < 4) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+      // (the shares' sum is what the block is launched with: 384 x 168, 512 x 128)
+      if constexpr (BITS4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+      else asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
       if (warp == 0) {
         // ---------------------------------------------------------------- TMA
         const int psb = min(1 << a.c.page_shift, kTBK);  // rows of a box
@@ -242,7 +276,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
         int it = 0, tc = 0;
         // a tile's boxes, one per page and 64 dims (at most 32: a lane issues one)
         auto load = [&](const CUtensorMap* map, int t, bool is_k) {
-          const int slot = it % kTSlots;
+          const int slot = it % NS;
           const int p = lane % pages, j = t * kTBK + p * psb;
           const bool in = j < g.keys;
           const int page = in ? a.table[g.b * a.table_stride + (j >> a.c.page_shift)] : -1;
@@ -250,12 +284,12 @@ __global__ void __launch_bounds__(kTThreads, 1)
           const uint32_t bad = __ballot_sync(0xffffffffu, in && lane < pages && !good);
           if (is_k) {
             if (lane == 0) {
-              s_pages[tc % kTOkRing] = ~bad;
+              s_pages[tc % kTOkRing][0] = ~bad;
               if (bad != 0) record_status(status, kDevBadPage);
             }
             ++tc;
           }
-          mbar_wait(&empty_bar[slot], ((it / kTSlots) & 1) ^ 1, status, abort_flag);
+          mbar_wait(&empty_bar[slot], ((it / NS) & 1) ^ 1, status, abort_flag);
           if (lane == 0) mbar_arrive_expect_tx(&full_bar[slot], TILE);
           __syncwarp();
           if (lane < boxes) {
@@ -268,7 +302,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
         while (__all_sync(0xffffffffu, next_segment(seg, g))) {
           if (lane == 0) mbar_arrive(&seg_empty[seg % kTSegs]);
           const int n = g.t1 - g.t0;
-          load(&tm_k, g.t0, true);
+          if constexpr (!BITS4) load(&tm_k, g.t0, true);
           mbar_wait(&q_empty, (seg & 1) ^ 1, status, abort_flag);
           if (lane == 0) {
             mbar_arrive_expect_tx(&q_full, a.tq * a.gs * (D / 64) * 128);
@@ -277,6 +311,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
           }
           __syncwarp();
           ++seg;
+          if constexpr (BITS4) continue;
           if constexpr (DUAL) {
             for (int t = g.t0; t < g.t1; ++t) {
               if (t > g.t0) load(&tm_k, t, true);
@@ -291,8 +326,8 @@ __global__ void __launch_bounds__(kTThreads, 1)
           }
         }
         // the copies into every slot have landed before the CTA may end
-        for (int i = max(0, it - kTSlots); i < it; ++i)
-          mbar_wait(&full_bar[i % kTSlots], (i / kTSlots) & 1, status, nullptr);
+        for (int i = max(0, it - NS); i < it; ++i)
+          mbar_wait(&full_bar[i % NS], (i / NS) & 1, status, nullptr);
         if (seg > 0) mbar_wait(&q_full, (seg - 1) & 1, status, nullptr);
       } else if (warp == 3) {
         // ---------------------------------------------------------------- segments
@@ -337,11 +372,11 @@ __global__ void __launch_bounds__(kTThreads, 1)
         constexpr uint32_t idesc_o = idesc_f16(kBF16, 128, D) | kIdescBMn;
         int it = 0, np[2] = {0, 0};
         auto wait_full = [&](int i) {
-          mbar_wait(&full_bar[i % kTSlots], (i / kTSlots) & 1, status, abort_flag);
+          mbar_wait(&full_bar[i % NS], (i / NS) & 1, status, abort_flag);
           tc_fence_after();
         };
         auto qk = [&](int i, int s) {  // S_s = Q_s K^T, K in the slot of step i
-          const uint32_t ks = ring_s + (i % kTSlots) * TILE, qs = q_s + (DUAL ? s * (128 * 128) : 0);
+          const uint32_t ks = ring_s + (i % NS) * TILE, qs = q_s + (DUAL ? s * (128 * 128) : 0);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t qo = (kk / 4) * C::QHALF + (kk % 4) * 32, ko = (kk / 4) * HALF + (kk % 4) * 32;
@@ -350,7 +385,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
         };
         // O_s (+)= P_s V, each half as soon as its 64 keys of P are there
         auto pv = [&](int i, int s, bool first) {
-          const uint32_t vs = ring_s + (i % kTSlots) * TILE;
+          const uint32_t vs = ring_s + (i % NS) * TILE;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             mbar_wait(&p_bar[s][h], np[s] & 1, status, abort_flag);
@@ -375,7 +410,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
             umma_commit(&s_bar[0]);
             qk(kslot, 1);
             umma_commit(&s_bar[1]);
-            umma_commit(&empty_bar[kslot % kTSlots]);
+            umma_commit(&empty_bar[kslot % NS]);
             if (n == 1) umma_commit(&q_empty);
             for (int t = 0; t < n; ++t) {
               const bool more = t + 1 < n;
@@ -391,11 +426,11 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 umma_commit(&o_bar[0]);
               }
               pv(vslot, 1, t == 0);
-              umma_commit(&empty_bar[vslot % kTSlots]);
+              umma_commit(&empty_bar[vslot % NS]);
               if (more) {
                 qk(kslot, 1);
                 umma_commit(&s_bar[1]);
-                umma_commit(&empty_bar[kslot % kTSlots]);
+                umma_commit(&empty_bar[kslot % NS]);
                 if (t + 2 == n) umma_commit(&q_empty);  // the segment's last product with Q
               } else {
                 umma_commit(&o_bar[1]);
@@ -405,7 +440,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
             for (int s = 0; s < min(n, 2); ++s) {
               wait_full(it);
               qk(it, s);
-              umma_commit(&empty_bar[it % kTSlots]);
+              umma_commit(&empty_bar[it % NS]);
               umma_commit(&s_bar[s]);
               ++it;
             }
@@ -414,12 +449,12 @@ __global__ void __launch_bounds__(kTThreads, 1)
               const int s = t & 1;
               wait_full(it);
               pv(it, s, t < 2);
-              umma_commit(&empty_bar[it % kTSlots]);
+              umma_commit(&empty_bar[it % NS]);
               ++it;
               if (t + 2 < n) {
                 wait_full(it);
                 qk(it, s);
-                umma_commit(&empty_bar[it % kTSlots]);
+                umma_commit(&empty_bar[it % NS]);
                 umma_commit(&s_bar[s]);
                 if (t + 3 == n) umma_commit(&q_empty);  // the segment's last product with Q
                 ++it;
@@ -432,9 +467,114 @@ __global__ void __launch_bounds__(kTThreads, 1)
         umma_commit(&drain_bar);
         mbar_wait(&drain_bar, 0, status, nullptr);
       }
+    } else if (BITS4 && warp >= 12) {
+      // ------------------------------------------------------------------ values of a 4-bit cache
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+      if constexpr (BITS4) {
+        constexpr int ROW = C::ROW4, CH = ROW / 16, G = D / 32;
+        const int w4 = warp - 12;  // this warp's 32 keys of a tile
+        uint8_t* raw = sm + C::Q + NS * TILE + C::GIVE + w4 * (kTRaw * 32 * ROW);
+        const uint32_t raw_s = smem_u32(raw);
+        const int page_mask = (1 << a.c.page_shift) - 1;
+        int it = 0, tc = 0;
+        while (__all_sync(0xffffffffu, next_segment(seg, g))) {
+          mbar_arrive(&seg_empty[seg % kTSegs]);
+          ++seg;
+          const int n = g.t1 - g.t0;
+          const int* table = a.table + g.b * a.table_stride;
+          // the page of this lane's key for step k (one step ahead of its loads)
+          auto look_up = [&](int k) {
+            if (k >= 2 * n) return -1;
+            int tile;
+            bool is_k;
+            load_step<DUAL>(n, k, tile, is_k);
+            const int j = (g.t0 + tile) * kTBK + w4 * 32 + lane;
+            return j < g.keys ? table[j >> a.c.page_shift] : -1;
+          };
+          int page = look_up(0);
+          auto issue = [&](int k) {
+            if (k < 2 * n) {
+              int tile;
+              bool is_k;
+              load_step<DUAL>(n, k, tile, is_k);
+              const int j = (g.t0 + tile) * kTBK + w4 * 32 + lane;
+              const bool in = j < g.keys, ok = in && page >= 0 && page < a.c.num_pages;
+              const long long off = ok ? page * a.c.page_stride + (j & page_mask) * a.c.token_stride : 0;
+              const uint32_t okm = __ballot_sync(0xffffffffu, ok);
+              if (is_k) {
+                if (in && !ok) record_status(status, kDevBadPage);
+                // (what lies behind the keys is masked by the keys' number)
+                const uint32_t lost = __ballot_sync(0xffffffffu, in && !ok);
+                if (lane == 0) s_pages[(tc + tile) % kTOkRing][w4] = ~lost;
+              }
+              page = look_up(k + 1);
+              const uint8_t* src = (is_k ? a.c.k : a.c.v) + g.kvh * a.c.head_stride;
+              const uint32_t dst = raw_s + (k % kTRaw) * (32 * ROW);
+#pragma unroll
+              for (int i = 0; i < CH; ++i) {
+                const int idx = i * 32 + lane, key = idx / CH, ch = idx % CH;
+                const long long o = __shfl_sync(0xffffffffu, off, key) + ch * 16;
+                cp_async16(dst + key * ROW + ch * 16, src + o, (okm >> key) & 1u);
+              }
+            }
+            cp_commit();
+          };
+#pragma unroll
+          for (int k = 0; k < kTRaw - 1; ++k) issue(k);
+#pragma unroll 1
+          for (int k = 0; k < 2 * n; ++k) {
+            cp_wait<kTRaw - 2>();
+            __syncwarp();
+            issue(k + kTRaw - 1);  // (into the slot that the last step left)
+            int tile;
+            bool is_k;
+            load_step<DUAL>(n, k, tile, is_k);
+            const int slot = it % NS;
+            mbar_wait(&empty_bar[slot], ((it / NS) & 1) ^ 1, status, abort_flag);
+            ++it;
+            const uint8_t* rows = raw + (k % kTRaw) * (32 * ROW);
+            uint8_t* out = sm + C::Q + slot * TILE;
+#pragma unroll 2
+            for (int i = 0; i < G; ++i) {
+              // eight lanes store to eight different 16-byte columns: two groups x four rows
+              int key, gr;
+              if (G == 4) {
+                key = i * 8 + ((lane >> 1) & 3) + ((lane >> 4) & 1) * 4;
+                gr = (lane & 1) + ((lane >> 3) & 1) * 2;
+              } else {
+                key = i * 16 + (lane >> 1);
+                gr = lane & 1;
+              }
+              const uint4 codes = *reinterpret_cast<const uint4*>(rows + key * ROW + gr * 16);
+              const uint32_t sz = *reinterpret_cast<const uint32_t*>(rows + key * ROW + D / 2 + gr * 4);
+              const uint32_t s2 = __byte_perm(sz, sz, 0x1010), z2 = __byte_perm(sz, sz, 0x3232);
+              const int r = w4 * 32 + key;
+              uint8_t* dst = out + (gr >> 1) * HALF + r * 128;
+              const uint32_t* cw = &codes.x;
+#pragma unroll
+              for (int wd = 0; wd < 4; ++wd) {
+                const uint32_t c = cw[wd];
+                const uint32_t p0 = H::dequant(nib<T, 0>(c), s2, z2), p1 = H::dequant(nib<T, 1>(c), s2, z2);
+                const uint32_t p2 = H::dequant(nib<T, 2>(c), s2, z2), p3 = H::dequant(nib<T, 3>(c), s2, z2);
+                uint4 v = make_uint4(p0, p1, p2, p3);
+                if (is_k)
+                  v = make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632),
+                                 __byte_perm(p2, p3, 0x7632));
+                *reinterpret_cast<uint4*>(dst + ((((gr & 1) * 4 + wd) ^ (r & 7)) << 4)) = v;
+              }
+            }
+            fence_async_proxy();
+            mbar_arrive(&full_bar[slot]);
+          }
+          cp_wait<0>();
+          __syncwarp();
+          tc += n;
+        }
+      }
     } else {
       // ------------------------------------------------------------------ softmax and output
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+      if constexpr (BITS4) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+      else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
       const int s = (warp - 4) >> 2;                  // stream
       const int row = (warp & 3) * 32 + lane;         // TMEM lane
       const int r = DUAL ? s * 128 + row : row;       // row of the row tile
@@ -473,8 +613,8 @@ __global__ void __launch_bounds__(kTThreads, 1)
           if (cut) {
             // V: what no mask stops from entering the product has to be finite
             const int vstep = it + (DUAL ? 2 * i + 1 : i + min(i + 2, n));
-            mbar_wait(&full_bar[vstep % kTSlots], (vstep / kTSlots) & 1, status, abort_flag);
-            uint4* vp = reinterpret_cast<uint4*>(sm + C::Q + (vstep % kTSlots) * TILE);
+            mbar_wait(&full_bar[vstep % NS], (vstep / NS) & 1, status, abort_flag);
+            uint4* vp = reinterpret_cast<uint4*>(sm + C::Q + (vstep % NS) * TILE);
             bool bad = false;
 #pragma unroll 4
             for (int c = 0; c < D / 8; ++c) {
@@ -505,8 +645,8 @@ __global__ void __launch_bounds__(kTThreads, 1)
             ++ns;
             continue;
           }
-          const uint32_t pages_ok = s_pages[(tc + i) % kTOkRing];
-          const bool masked = cut || pages_ok != 0xffffffffu;
+          const uint32_t* ok = s_pages[(tc + i) % kTOkRing];  // a bit per page, or per key of a 4-bit cache
+          const bool masked = cut || (BITS4 ? (ok[0] & ok[BITS4 ? 1 : 0] & ok[BITS4 ? 2 : 0] & ok[BITS4 ? 3 : 0]) : ok[0]) != 0xffffffffu;
           uint32_t x[4][32];
 #pragma unroll
           for (int q = 0; q < 4; ++q) tmem_ld32_issue(t_s + q * 32, x[q]);
@@ -532,9 +672,11 @@ __global__ void __launch_bounds__(kTThreads, 1)
                   const uint32_t hi = w0 + 1 < a.tree_words ? static_cast<uint32_t>(words[w0 + 1]) : 0u;
                   see &= __funnelshift_r(lo, hi, sh);
                 }
-                if (pages_ok != 0xffffffffu) {
+                if constexpr (BITS4) {
+                  see &= ok[q];
+                } else if (ok[0] != 0xffffffffu) {
                   for (int e = 0; e < 32; ++e)
-                    if (!((pages_ok >> ((q * 32 + e) / psb)) & 1u)) see &= ~(1u << e);
+                    if (!((ok[0] >> ((q * 32 + e) / psb)) & 1u)) see &= ~(1u << e);
                 }
               }
 #pragma unroll
@@ -609,7 +751,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
         const long long slot = g.slot;
         float f_own = 1.f, f_other = 0.f;
         if constexpr (!DUAL) {
-          float2* ml = reinterpret_cast<float2*>(sm + C::Q + kTSlots * TILE);
+          float2* ml = reinterpret_cast<float2*>(sm + C::Q + NS * TILE);
           ml[s * 128 + row] = make_float2(m, l);
           both();
           const float2 o = ml[(s ^ 1) * 128 + row];
@@ -642,12 +784,21 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 if (!visible(j)) continue;
                 const int page = a.table[g.b * a.table_stride + (j >> a.c.page_shift)];
                 if (page < 0 || page >= a.c.num_pages) continue;
-                const T* v = reinterpret_cast<const T*>(a.c.v + page * a.c.page_stride + g.kvh * a.c.head_stride +
-                                                        (j & ((1 << a.c.page_shift) - 1)) * a.c.token_stride) + q * 32;
+                const uint8_t* v = a.c.v + page * a.c.page_stride + g.kvh * a.c.head_stride +
+                                   (j & ((1 << a.c.page_shift) - 1)) * a.c.token_stride;
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
-                  const float f = to_f32<T>(v[e]);
-                  if (!isfinite(f)) o[e] = __float_as_uint(__uint_as_float(o[e]) + f);
+                  float f;
+                  int at = e;
+                  if constexpr (BITS4) {
+                    const T* sz = reinterpret_cast<const T*>(v + D / 2 + q * 4);
+                    const int code = (v[q * 16 + e / 2] >> (4 * (e & 1))) & 15;
+                    f = to_f32<T>(from_f32<T>(fmaf(static_cast<float>(code), to_f32<T>(sz[0]), to_f32<T>(sz[1]))));
+                    at = (e & ~7) + nibble_place(e & 7);
+                  } else {
+                    f = to_f32<T>(reinterpret_cast<const T*>(v)[q * 32 + e]);
+                  }
+                  if (!isfinite(f)) o[at] = __float_as_uint(__uint_as_float(o[at]) + f);
                 }
               }
             }
@@ -656,21 +807,22 @@ __global__ void __launch_bounds__(kTThreads, 1)
         };
         auto store_o = [&](int q, const uint32_t (&o)[32]) {
           if (!row_ok) return;
+          auto col = [&](int d) { return __uint_as_float(o[BITS4 ? (d & ~7) + nibble_place(d & 7) : d]); };
           if (whole) {
             uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + q * 32);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               uint4 v;
-              v.x = H::pack(__uint_as_float(o[8 * c]) * inv, __uint_as_float(o[8 * c + 1]) * inv);
-              v.y = H::pack(__uint_as_float(o[8 * c + 2]) * inv, __uint_as_float(o[8 * c + 3]) * inv);
-              v.z = H::pack(__uint_as_float(o[8 * c + 4]) * inv, __uint_as_float(o[8 * c + 5]) * inv);
-              v.w = H::pack(__uint_as_float(o[8 * c + 6]) * inv, __uint_as_float(o[8 * c + 7]) * inv);
+              v.x = H::pack(col(8 * c) * inv, col(8 * c + 1) * inv);
+              v.y = H::pack(col(8 * c + 2) * inv, col(8 * c + 3) * inv);
+              v.z = H::pack(col(8 * c + 4) * inv, col(8 * c + 5) * inv);
+              v.w = H::pack(col(8 * c + 6) * inv, col(8 * c + 7) * inv);
               dst[c] = v;
             }
           } else {
             float* dst = a.part_o + (slot * D + q * 32) * R + r;  // rows innermost: a warp's store is one line
 #pragma unroll
-            for (int e = 0; e < 32; ++e) dst[e * R] = __uint_as_float(o[e]);
+            for (int e = 0; e < 32; ++e) dst[e * R] = col(e);
           }
         };
         if constexpr (DUAL) {
@@ -683,8 +835,8 @@ __global__ void __launch_bounds__(kTThreads, 1)
         } else {
           // each stream finishes half of the columns: it leaves the other's, 32 at a time, as [column][row]
           constexpr int HQ = D / 64;
-          float* give = reinterpret_cast<float*>(sm + C::Q + kTSlots * TILE) + s * (32 * 128);
-          const float* take = reinterpret_cast<const float*>(sm + C::Q + kTSlots * TILE) + (s ^ 1) * (32 * 128);
+          float* give = reinterpret_cast<float*>(sm + C::Q + NS * TILE) + s * (32 * 128);
+          const float* take = reinterpret_cast<const float*>(sm + C::Q + NS * TILE) + (s ^ 1) * (32 * 128);
 #pragma unroll 1
           for (int q = 0; q < HQ; ++q) {
             uint32_t o[32];
@@ -724,13 +876,24 @@ __global__ void __launch_bounds__(kTThreads, 1)
   if (warp == 2) tmem_dealloc(tmem, 512);
 }
 
-template <int D, bool DUAL>
-const void* tc_fn(bool bf16) {
-  return bf16 ? reinterpret_cast<const void*>(paged_attn_tc_kernel<D, DUAL, __nv_bfloat16>)
-              : reinterpret_cast<const void*>(paged_attn_tc_kernel<D, DUAL, __half>);
+struct Variant {
+  const void* fn;
+  int smem, threads;
+};
+template <int D, bool DUAL, bool BITS4>
+Variant variant(bool bf16) {
+  using C = TcCfg<D, DUAL, BITS4>;
+  return {bf16 ? reinterpret_cast<const void*>(paged_attn_tc_kernel<D, DUAL, BITS4, __nv_bfloat16>)
+               : reinterpret_cast<const void*>(paged_attn_tc_kernel<D, DUAL, BITS4, __half>),
+          C::SMEM, C::THREADS};
+}
+template <int D>
+Variant variant(bool dual, bool bits4, bool bf16) {
+  if (dual) return bits4 ? variant<D, true, true>(bf16) : variant<D, true, false>(bf16);
+  return bits4 ? variant<D, false, true>(bf16) : variant<D, false, false>(bf16);
 }
 
-std::atomic<int> g_smem_seen[8][64];
+std::atomic<int> g_smem_seen[16][64];
 
 bool encode(CUtensorMap* map, const void* base, bool bf16, int rank, const cuuint64_t* dims, cuuint64_t* strides,
             const cuuint32_t* box) {
@@ -766,12 +929,12 @@ bool encode_queries(CUtensorMap* map, const AttnArgs& a, int D, bool bf16) {
 
 }  // namespace
 
-bool tc_takes(const PagedCacheArgs& c) {
-  return c.page_shift >= 3 && c.num_pages >= 1 && c.num_pages < 0x7fffffffll;
+bool tc_takes(const PagedCacheArgs& c, bool bits4) {
+  return bits4 || (c.page_shift >= 3 && c.num_pages >= 1 && c.num_pages < 0x7fffffffll);
 }
 
-bool plan_attn_tc(int N, int B, int g, int D, bool bits4, int sms, AttnPlan* p) {
-  if (bits4 || D > 128 || g > 128) return false;
+bool plan_attn_tc(int N, int B, int g, int D, int sms, AttnPlan* p) {
+  if (D > 128 || g > 128) return false;
   const long long rows = (static_cast<long long>(N) * g + B - 1) / B;
   if (rows <= kTcMinRows) return false;
   p->rows = rows > 128 ? 256 : 128;
@@ -781,21 +944,24 @@ bool plan_attn_tc(int N, int B, int g, int D, bool bits4, int sms, AttnPlan* p) 
   return true;
 }
 
-cudaError_t launch_attn_tc(AttnArgs a, const AttnPlan& p, int D, bool bf16, cudaStream_t stream, bool pdl, bool* fits) {
+cudaError_t launch_attn_tc(AttnArgs a, const AttnPlan& p, int D, bool bf16, bool bits4, cudaStream_t stream, bool pdl,
+                           bool* fits) {
   CUtensorMap tq, tk, tv;
-  *fits = encode_queries(&tq, a, D, bf16) && encode_cache(&tk, a.c, a.c.k, D, bf16) && encode_cache(&tv, a.c, a.c.v, D, bf16);
+  *fits = encode_queries(&tq, a, D, bf16);
+  if (bits4) {
+    tk = tv = tq;  // (not used)
+  } else {
+    *fits = *fits && encode_cache(&tk, a.c, a.c.k, D, bf16) && encode_cache(&tv, a.c, a.c.v, D, bf16);
+  }
   if (!*fits) return cudaSuccess;
   const bool dual = p.rows == 256;
-  const void* fn = D == 64 ? (dual ? tc_fn<64, true>(bf16) : tc_fn<64, false>(bf16))
-                           : (dual ? tc_fn<128, true>(bf16) : tc_fn<128, false>(bf16));
-  const int smem = D == 64 ? (dual ? TcCfg<64, true>::SMEM : TcCfg<64, false>::SMEM)
-                           : (dual ? TcCfg<128, true>::SMEM : TcCfg<128, false>::SMEM);
-  cudaError_t err = ensure_dyn_smem(fn, smem, g_smem_seen[(D == 128) * 4 + dual * 2 + bf16], 64);
+  const Variant v = D == 64 ? variant<64>(dual, bits4, bf16) : variant<128>(dual, bits4, bf16);
+  cudaError_t err = ensure_dyn_smem(v.fn, v.smem, g_smem_seen[(D == 128) * 8 + dual * 4 + bits4 * 2 + bf16], 64);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.grid);
-  cfg.blockDim = dim3(kTThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3(v.threads);
+  cfg.dynamicSmemBytes = v.smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -803,7 +969,7 @@ cudaError_t launch_attn_tc(AttnArgs a, const AttnPlan& p, int D, bool bf16, cuda
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
   void* params[] = {&a, &tq, &tk, &tv};
-  err = cudaLaunchKernelExC(&cfg, fn, params);
+  err = cudaLaunchKernelExC(&cfg, v.fn, params);
   if (err != cudaSuccess) return err;
   return launch_attn_join(a, p, D, bf16, stream, pdl);
 }

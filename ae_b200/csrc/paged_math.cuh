@@ -103,4 +103,13 @@ __device__ __forceinline__ uint32_t nib(uint32_t w) {
   return (v & Half2<T>::kMask) | Half2<T>::kBase;
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool fill) {
+  const int n = fill ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 }  // namespace smb

@@ -56,8 +56,9 @@ def head_norm(x, w, eps):
 
 
 def attention(q, k_cache, v_cache, table, kv_lens, q_starts, tree=None, scale=None, pages_ok=None):
-    """(out, lse, spread): out [N, Hq, D] and lse [N, Hq] in 64 bits, NaN in rows of no sequence;
-    spread [N, Hq, D] = sum_j p_j |v_j|, what roundings of p and v are relative to."""
+    """(out, lse, spread, reach): out [N, Hq, D] and lse [N, Hq] in 64 bits, NaN in rows of no sequence;
+    spread [N, Hq, D] = sum_j p_j |v_j|, what roundings of p and v are relative to; reach [N, Hq] =
+    max_j scale sum_d |q_d k_jd|, what roundings of k are relative to."""
     dtype = q.dtype
     N, Hq, D = q.shape
     P, Hkv, ps, _ = k_cache.shape
@@ -65,6 +66,7 @@ def attention(q, k_cache, v_cache, table, kv_lens, q_starts, tree=None, scale=No
     out = torch.full((N, Hq, D), math.nan, dtype=torch.float64, device=q.device)
     spread = out.clone()
     lse = torch.full((N, Hq), math.nan, dtype=torch.float64, device=q.device)
+    reach = torch.zeros((N, Hq), dtype=torch.float64, device=q.device)
     starts, lens = q_starts.tolist(), kv_lens.tolist()
     for b in range(len(lens)):
         s0, s1 = starts[b], min(starts[b + 1], N)
@@ -98,7 +100,8 @@ def attention(q, k_cache, v_cache, table, kv_lens, q_starts, tree=None, scale=No
                     continue
                 sc = q[s0 + i, hs].double() @ Ks[:, h].T * scale
                 p = torch.softmax(sc, -1)
+                reach[s0 + i, hs] = (q[s0 + i, hs].double().abs() @ Ks[:, h].abs().T).amax(-1) * scale
                 lse[s0 + i, hs] = torch.logsumexp(sc, -1)
                 out[s0 + i, hs] = p @ Vs[:, h]
                 spread[s0 + i, hs] = p @ Vs[:, h].abs()
-    return out, lse, spread
+    return out, lse, spread, reach
