@@ -333,6 +333,7 @@ __global__ void __launch_bounds__(BITS4 ? kTThreads4 : kTThreads, 1)
         // ---------------------------------------------------------------- segments
         Work k;
         bool more = work_begin<kTBK>(a, plan, W, cta, gridDim.x, k);
+        __syncwarp();  // (the first segment gives the plan's place to the ring: every lane has read it)
         if (!more && lane == 0) leave_record(a, cta, k);
         while (more) {
           const Cursor& cur = k.cur;
@@ -610,8 +611,11 @@ __global__ void __launch_bounds__(BITS4 ? kTThreads4 : kTThreads, 1)
         for (int i = DUAL ? 0 : s; i < n; i += DUAL ? 1 : 2) {
           const int j0 = (g.t0 + i) * kTBK;
           const bool cut = j0 + kTBK > g.open || j0 + kTBK > g.keys;
+          mbar_wait(&s_bar[s], ns & 1, status, abort_flag);
+          tc_fence_after();
           if (cut) {
-            // V: what no mask stops from entering the product has to be finite
+            // V: what no mask stops from entering the product has to be finite.  (S being there says that
+            // what its slot held before has been used, so that the wait can only be for this V.)
             const int vstep = it + (DUAL ? 2 * i + 1 : i + min(i + 2, n));
             mbar_wait(&full_bar[vstep % NS], (vstep / NS) & 1, status, abort_flag);
             uint4* vp = reinterpret_cast<uint4*>(sm + C::Q + (vstep % NS) * TILE);
@@ -637,8 +641,6 @@ __global__ void __launch_bounds__(BITS4 ? kTThreads4 : kTThreads, 1)
             }
             if (bad) fence_async_proxy();
           }
-          mbar_wait(&s_bar[s], ns & 1, status, abort_flag);
-          tc_fence_after();
           if (!some) {  // nothing to weigh: the product may have what is there
             mbar_arrive(&p_bar[s][0]);
             mbar_arrive(&p_bar[s][1]);
