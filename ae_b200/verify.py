@@ -10,6 +10,11 @@ token sees the cache, its ancestors and itself) -> RMSNorm -> MoE block (gate + 
 (``mixtral.py:226-268``); then the final norm, the LM head and greedy acceptance of the
 draft tree.  Weights are random (no checkpoints); shapes follow Mixtral-8x7B.
 
+The keys and values sit in one dense tensor per layer with torch operations around them
+(``cache="dense"``, the default, on any device), or in a paged cache, of 16-bit values
+(``"paged"``) or 4-bit codes (``"paged4"``), with rotation, cache write and attention by the
+library (``ae_b200.paged``: two calls per layer).
+
 The MoE calls can be bracketed by CUDA events (``moe_events``) so that the MoE layers'
 share of the step is measured on the device.
 """
@@ -21,7 +26,7 @@ from typing import Callable, List, Optional
 
 import torch
 
-from . import ops
+from . import ops, paged
 
 
 @dataclasses.dataclass(frozen=True)
@@ -88,10 +93,16 @@ class VerifyDecoder:
 
     ``moe`` computes one MoE block in place: ``moe(layer, h [N, H]) -> h``; by default the
     sm_100a library (gate fused into the routing launch).  The expert pools are held per
-    layer on the device: ``pools[l]`` [E, 3*I*H], page table identity."""
+    layer on the device: ``pools[l]`` [E, 3*I*H], page table identity.
+
+    ``cache``: "dense", "paged" or "paged4", with pages of ``page_size`` tokens; the same seed
+    gives the same weights and cached values for each (rounded to 4 bits by the last)."""
 
     def __init__(self, cfg: DecoderConfig, batch: int, cache_len: int, max_draft: int, device,
-                 dtype=torch.bfloat16, seed: int = 0, moe: Optional[Callable] = None):
+                 dtype=torch.bfloat16, seed: int = 0, moe: Optional[Callable] = None, cache: str = "dense",
+                 page_size: int = 64):
+        if cache not in ("dense", "paged", "paged4"):
+            raise ValueError(f"cache must be dense, paged or paged4, got {cache!r}")
         self.cfg, self.batch, self.cache_len, self.max_draft = cfg, batch, cache_len, max_draft
         self.device = torch.device(device)
         self.dtype = dtype
@@ -123,6 +134,48 @@ class VerifyDecoder:
         self.k_cache = [rnd(batch, c.kv_heads, S, c.head_dim, std=1.0) for _ in range(c.layers)]
         self.v_cache = [rnd(batch, c.kv_heads, S, c.head_dim, std=1.0) for _ in range(c.layers)]
         self.moe = moe or self._library_moe
+        self.cache = cache
+        if cache != "dense":
+            self._page_caches(page_size, 4 if cache == "paged4" else 16)
+
+    def _page_caches(self, page_size: int, bits: int):
+        """Moves the dense caches into pages (in an order of their own for each layer's cache alike)."""
+        c, B, n = self.cfg, self.batch, self.cache_len
+        S = n + self.max_draft
+        per = -(-S // page_size)
+        g = torch.Generator().manual_seed(0)
+        self.block_table = torch.randperm(B * per, generator=g).view(B, per).to(torch.int32).to(self.device)
+        places = torch.arange(per * page_size, device=self.device)
+        self.slots = (self.block_table.long()[:, places // page_size] * page_size + places % page_size)  # [B, places]
+        self.inv_freq, _ = paged.rope_inv_freq(c.head_dim, c.rope_theta, device=self.device)
+        for li in range(c.layers):
+            k, v = (t.transpose(1, 2)[:, :n].reshape(B * n, c.kv_heads, c.head_dim).contiguous()
+                    for t in (self.k_cache[li], self.v_cache[li]))
+            kc, vc = paged.new_cache(B * per, c.kv_heads, page_size, c.head_dim, self.dtype, self.device, bits)
+            if n > 0:
+                paged.kv_append(k, k, v, kc, vc, self.slots[:, :n].reshape(-1).contiguous())
+            self.k_cache[li], self.v_cache[li] = kc, vc
+
+    def _paged_attention(self, layer: int, h: torch.Tensor, step: dict) -> torch.Tensor:
+        """``attention`` over the paged cache: rotate and append, then attend."""
+        c, L = self.cfg, self.layers[layer]
+        B, n, _ = h.shape
+        x = (h @ L["wqkv"].t()).view(B * n, c.heads + 2 * c.kv_heads, c.head_dim)
+        q, k, v = x[:, :c.heads], x[:, c.heads:c.heads + c.kv_heads], x[:, c.heads + c.kv_heads:]
+        kc, vc = self.k_cache[layer], self.v_cache[layer]
+        q = paged.kv_append(q, k, v, kc, vc, step["slots"], step["positions"], self.inv_freq)
+        o = paged.paged_attention(q, kc, vc, self.block_table, step["kv_lens"], step["q_starts"], tree=step["tree"])
+        return o.view(B, n, c.heads * c.head_dim) @ L["wo"].t()
+
+    def _paged_step(self, parents: List[int]) -> dict:
+        """What the layers of one step share: slots, positions, lengths and the trees' words."""
+        B, n = self.batch, len(parents)
+        pos = torch.tensor(tree_depths(parents), device=self.device) + self.cache_len
+        return {"slots": self.slots[:, self.cache_len:self.cache_len + n].reshape(-1).contiguous(),
+                "positions": pos.repeat(B),
+                "kv_lens": torch.full((B,), self.cache_len + n, dtype=torch.int32, device=self.device),
+                "q_starts": torch.arange(0, (B + 1) * n, n, dtype=torch.int32, device=self.device),
+                "tree": paged.tree_words([parents] * B).to(self.device)}
 
     def _library_moe(self, layer: int, h: torch.Tensor) -> torch.Tensor:
         L = self.layers[layer]
@@ -158,12 +211,18 @@ class VerifyDecoder:
         B, n = tokens.shape
         if n > self.max_draft:
             raise ValueError("more draft tokens than the cache has room for")
-        mask = tree_mask(parents).to(self.device)
-        pos = torch.tensor(tree_depths(parents), device=self.device) + self.cache_len
+        if len(parents) != n:
+            raise ValueError("parents must have an entry for each draft token")
+        if self.cache == "dense":
+            mask = tree_mask(parents).to(self.device)
+            pos = torch.tensor(tree_depths(parents), device=self.device) + self.cache_len
+        else:
+            step = self._paged_step(parents)
         h = self.embed[tokens]
         for li in range(c.layers):
             L = self.layers[li]
-            h = h + self.attention(li, rms_norm(h, L["norm1"], c.eps), pos, mask)
+            x = rms_norm(h, L["norm1"], c.eps)
+            h = h + (self.attention(li, x, pos, mask) if self.cache == "dense" else self._paged_attention(li, x, step))
             y = rms_norm(h, L["norm2"], c.eps).reshape(B * n, c.H).contiguous()
             if moe_events is not None:
                 moe_events[li][0].record()

@@ -468,3 +468,101 @@ def test_no_tokens_and_no_sequences():
     kv = torch.zeros(0, 2, 64, dtype=BF, device="cuda")
     q = paged.kv_append(e, kv, kv, d["k_cache"], d["v_cache"], torch.zeros(0, dtype=torch.int64, device="cuda"))
     assert q.shape == (0, 4, 64)
+
+
+def test_same_bits_again_and_again():
+    """Every kernel path, repeated among other work: the same bits each time."""
+    picks = [0, 3, 5, 6, 10, 11, 13, 14, 15, 16, 17, 18, 20]
+    cases = []
+    for bits in (16, 4):
+        for i in picks:
+            new, keys, Hq, Hkv, D, ps, tree = SHAPES[i]
+            cases.append(make_batch(new, keys, Hq, Hkv, D, ps, BF if i % 2 else FP, bits, tree, seed=i))
+    first = [call(d) for d in cases]
+    junk = torch.empty(16 << 20, device="cuda")
+    for r in range(25):
+        for n, d in enumerate(cases):
+            out, lse = call(d)
+            assert torch.equal(out, first[n][0]) and torch.equal(lse, first[n][1]), (n, r)
+            if n % 5 == r % 5:
+                junk.fill_(math.nan)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams overlap without a shared workspace."""
+    cases = [make_batch([32] * 4, [900, 33, 2000, 64], 8, 2, 128, 16, BF, bits, True, seed=bits) for bits in (16, 4)]
+    want = [call(d) for d in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (d, s) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(call(d))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out, lse in got[i]:
+            assert torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])
+
+
+def test_long_rows_of_scores_far_apart():
+    """Scores that grow along the keys by hundreds: every tile raises the maximum."""
+    for bits, heads in ((16, 4), (16, 64), (4, 4)):
+        d = make_batch([2], [700], heads, 2, 128, 16, BF, bits, False, seed=1)
+        if bits == 16:
+            ramp = torch.linspace(-3, 3, d["k_cache"].shape[0] * 16, device="cuda").view(-1, 1, 16, 1)
+            d["k_cache"] = (d["k_cache"] * 0.1 + d["q"][0, 0] * ramp).to(BF)
+        d["q"] = (d["q"] * 6).to(BF)
+        out, lse = call(d)
+        o, l, spread, _ = ref.attention(d["q"], d["k_cache"], d["v_cache"], d["block_table"], d["kv_lens"], d["q_starts"])
+        # scores of up to a thousand: 32 bits hold them to 2^-14
+        u = ref.half_step(BF)
+        assert bool(((out.double() - o).abs() <= 2 * u * spread + u * o.abs() + 2 ** -11 * spread + 2 ** -25).all())
+        assert bool(((lse.double() - l).abs() <= 2 ** -17 * l.abs() + 2 ** -13).all())
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=lambda d: d["q"].float()), dict(q=lambda d: d["q"][:, 0]), dict(q=lambda d: d["q"][..., :64]),
+    dict(q=lambda d: d["q"].transpose(1, 2).contiguous().transpose(1, 2)), dict(q=lambda d: d["q"][:, :3]),
+    dict(k_cache=lambda d: d["k_cache"][:, :, :12]), dict(k_cache=lambda d: d["k_cache"].half()),
+    dict(k_cache=lambda d: d["k_cache"].transpose(1, 2).contiguous().transpose(1, 2)),
+    dict(block_table=lambda d: d["block_table"].long()), dict(block_table=lambda d: d["block_table"].cpu()),
+    dict(kv_lens=lambda d: d["kv_lens"].long()), dict(kv_lens=lambda d: d["kv_lens"][:1]),
+    dict(q_starts=lambda d: d["q_starts"][:2]), dict(q_starts=lambda d: d["q_starts"].cpu()),
+    dict(tree=lambda d: torch.zeros(3, 1, dtype=torch.int32, device="cuda")),
+    dict(tree=lambda d: torch.zeros(4, 0, dtype=torch.int32, device="cuda")),
+    dict(tree=lambda d: torch.zeros(4, 1, dtype=torch.int64, device="cuda"))])
+def test_attention_refusals(change):
+    from ae_b200 import paged
+    d = make_batch([3, 1], [40, 7], 4, 2, 128, 16, BF, 16, False)
+    for name, f in change.items():
+        d[name] = f(d)
+    with pytest.raises((ValueError, NotImplementedError)):
+        paged.paged_attention(**d)
+
+
+@pytest.mark.parametrize("kw", [dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan),
+                                dict(lse=torch.zeros(4, 4)), dict(out=torch.zeros(4, 4, 128)),
+                                dict(status=torch.zeros(1))])
+def test_attention_option_refusals(kw):
+    from ae_b200 import paged
+    d = make_batch([3, 1], [40, 7], 4, 2, 128, 16, BF, 16, False)
+    with pytest.raises(ValueError):
+        paged.paged_attention(**d, **kw)
+
+
+@pytest.mark.parametrize("change", [
+    dict(k=lambda c: c["k"][:, :1]), dict(v=lambda c: c["v"].float()), dict(slots=lambda c: c["slots"].int()),
+    dict(slots=lambda c: c["slots"][:-1]), dict(positions=lambda c: c["positions"].int()),
+    dict(inv_freq=lambda c: c["inv_freq"].float()), dict(inv_freq=lambda c: c["inv_freq"][:5]),
+    dict(inv_freq=lambda c: None), dict(inv_freq=lambda c: torch.ones(64, dtype=torch.float64, device="cuda")),
+    dict(q=lambda c: c["x"][:, :4, 1:]), dict(q=lambda c: c["q"].cpu()), dict(k_cache=lambda c: c["k_cache"][:1]),
+    dict(out=lambda c: torch.zeros(6, 4, 64, device="cuda")), dict(q_norm=lambda c: torch.ones(32, device="cuda"))])
+def test_append_refusals(change):
+    from ae_b200 import paged
+    c = append_case(0, BF, 16, 6, 4, 2, 64, 16, 64, False, False)
+    for name, f in change.items():
+        c[name] = f(c)
+    c.pop("x"), c.pop("w")
+    with pytest.raises((ValueError, NotImplementedError)):
+        paged.kv_append(**c)
