@@ -232,8 +232,11 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 8) kv_append_kernel(const _
         uint32_t codes = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
+          // the quotient corrected by its remainder: values of 16 bits meet the middle between two codes
+          // often, and a quotient off by a last place would round the wrong way there
+          const float x = v[e] - zero, q = x * inv;
           // the code's integer in the low bits of 2^23 + code (round to nearest even); NaN gives 0
-          const float c = fminf(fmaxf((v[e] - zero) * inv, 0.f), 15.f) + 8388608.f;
+          const float c = fminf(fmaxf(fmaf(fmaf(-q, scale, x), inv, q), 0.f), 15.f) + 8388608.f;
           codes |= (__float_as_uint(c) & 15u) << (4 * e);
         }
         if (there) {
