@@ -96,6 +96,9 @@ struct AttnPlan {
 };
 AttnPlan plan_attn_mma(int N, int B, int g, int D, bool bits4, int sms);
 cudaError_t launch_attn_mma(AttnArgs a, const AttnPlan& p, int D, bool bf16, bool bits4, cudaStream_t stream, bool pdl);
+// 4-bit caches and at most 8 query rows of a key head on average (false otherwise)
+bool plan_attn_q4(int N, int B, int g, int D, int sms, AttnPlan* p);
+cudaError_t launch_attn_q4(AttnArgs a, const AttnPlan& p, int D, bool bf16, cudaStream_t stream, bool pdl);
 // tcgen05 kernel: plan_attn_tc is false for few rows and heads of 256, tc_takes for 16-bit caches with
 // pages below 8 tokens.  launch_attn_tc leaves *fits false, and launches nothing, when strides do not
 // make a tensor map.

@@ -151,6 +151,7 @@ size_t smb_paged_attention_workspace_bytes(int N, int B, int Hq, int Hkv, int he
   size_t n = attn_ws(plan_attn_mma(N, B, g, head_dim, bits == 4, di.sms), head_dim);
   AttnPlan p;
   if (plan_attn_tc(N, B, g, head_dim, di.sms, &p)) n = std::max(n, attn_ws(p, head_dim));
+  if (bits == 4 && plan_attn_q4(N, B, g, head_dim, di.sms, &p)) n = std::max(n, attn_ws(p, head_dim));
   return n;
 }
 
@@ -217,6 +218,10 @@ int smb_paged_attention(const smb_attention_args_t* r, smb_stream_t stream) {
     bool fits = false;
     const cudaError_t err = launch_attn_tc(a, p, D, bf16, bits4, st, pdl_enabled(), &fits);
     if (err != cudaSuccess || fits) return done(err);
+  }
+  if (bits4 && plan_attn_q4(N, B, a.g, D, di.sms, &p)) {
+    if (!use()) return SMB_ERR_WORKSPACE;
+    return done(launch_attn_q4(a, p, D, bf16, st, pdl_enabled()));
   }
   p = plan_attn_mma(N, B, a.g, D, bits4, di.sms);
   if (!use()) return SMB_ERR_WORKSPACE;
