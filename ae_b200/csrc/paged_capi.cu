@@ -79,6 +79,7 @@ int smb_kv_append(const smb_append_args_t* p, smb_stream_t stream) {
   if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->q_out) || !aligned16(p->q_norm) ||
       !aligned16(p->k_norm))
     return SMB_ERR_ALIGN;
+  if (p->q_out == p->q) return SMB_ERR_ALIGN;
   for (int i = 0; i < 2; ++i)
     if (p->q_strides[i] % 8 != 0 || p->k_strides[i] % 8 != 0 || p->v_strides[i] % 8 != 0) return SMB_ERR_ALIGN;
   DeviceInfo di;
@@ -172,6 +173,8 @@ int smb_paged_attention(const smb_attention_args_t* r, smb_stream_t stream) {
   if (r->q == nullptr || r->out == nullptr || r->kv_lens == nullptr || r->q_starts == nullptr || r->ws == nullptr)
     return SMB_ERR_NULL;
   if (r->max_pages > 0 && r->block_table == nullptr) return SMB_ERR_NULL;
+  if (a.c.num_pages == 0) return SMB_ERR_SHAPE;
+  if (r->out == r->q) return SMB_ERR_ALIGN;
   if (!aligned16(r->q) || !aligned16(r->out) || !aligned16(r->ws)) return SMB_ERR_ALIGN;
   for (int i = 0; i < 2; ++i)
     if (r->q_strides[i] % 8 != 0 || r->out_strides[i] % 8 != 0) return SMB_ERR_ALIGN;

@@ -247,6 +247,8 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
         out = q.new_empty(shape)
     elif out.shape != shape or out.dtype != dtype or out.get_device() != dev or not out.is_contiguous():
         raise ValueError("out must be contiguous, with the shape, dtype and device of q")
+    elif N > 0 and out.data_ptr() == q.data_ptr():
+        raise ValueError("out may not be q")
     word, mine = _status_word(status, dev)
     args = _native.APPEND_ARGS
     rc = _launch(dev, _native.load().smb_kv_append, args.pack(
@@ -326,7 +328,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             tree_p = 0
     if out is None:
         out = q.new_empty(shape)
+    elif N > 0 and out.data_ptr() == q.data_ptr():
+        raise ValueError("out may not be q")
     ots, ohs = _rows("out", out, shape, dtype, dev)
+    if N > 0 and B > 0 and cache[2] == 0:
+        raise ValueError("the cache has no pages")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (N, Hq) or lse.get_device() != dev
                             or not lse.is_contiguous()):
         raise ValueError("lse must be contiguous float32 [N, Hq] on the device of q")

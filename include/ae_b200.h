@@ -394,7 +394,7 @@ SMB_API int smb_kv4_row_bytes(int head_dim);
  * 118-224 rotates and caches in separate kernels).  Strides {token, head} in elements, multiples of
  * 8; head_dim is contiguous.  A negative slot is not written; a slot past the cache is not written
  * and recorded as 2 in *status (device int, NULL: not recorded).  The slots of a call have to be
- * distinct. */
+ * distinct; q_out may not overlap q. */
 typedef struct smb_append_args {
   size_t struct_bytes; /* sizeof(smb_append_args_t) */
   smb_paged_cache_t cache;
@@ -427,7 +427,7 @@ SMB_API size_t smb_paged_attention_workspace_bytes(int N, int B, int Hq, int Hkv
  * or, given `tree` [N][tree_words] of 32 bits each, if j < P or bit j - P of its words is set (draft
  * trees: ancestors and itself; bits beyond the words read as 0).  out = softmax(scale * q k) v,
  * lse [N, Hq] (optional) = the natural log of the softmax's sum; a token that sees no key gets 0 and
- * -inf.  Rows of q that belong to no sequence leave out and lse as they were; out may not overlap q.
+ * -inf.  Rows of q that belong to no sequence leave out and lse as they were; out may not overlap q (SMB_ERR_ALIGN for q itself).
  * Lengths are read on the device: kv_lens is cut to max_pages * page_size, q_starts to [0, N]; keys of
  * a page outside [0, num_pages) are left out and recorded as 2 in *status (device int, optional).
  * (specmoe/layers/attention_backend/triton_backend.py, cpu_backend.py; the lse is what joins a

@@ -571,6 +571,11 @@ def test_attention_option_refusals(kw):
     d = make_batch([3, 1], [40, 7], 4, 2, 128, 16, BF, 16, False)
     with pytest.raises(ValueError):
         paged.paged_attention(**d, **kw)
+    with pytest.raises(ValueError):
+        paged.paged_attention(**d, out=d["q"])
+    d["k_cache"], d["v_cache"] = d["k_cache"][:0], d["v_cache"][:0]
+    with pytest.raises(ValueError):
+        paged.paged_attention(**d)
 
 
 @pytest.mark.parametrize("change", [

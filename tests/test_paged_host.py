@@ -158,7 +158,7 @@ def test_c_abi_refuses_bad_caches(lib, bad, code):
     (dict(struct_bytes=8), SHAPE), (dict(dtype=2), DTYPE), (dict(N=-1), SHAPE), (dict(Hq=0), SHAPE), (dict(Hq=2000), SHAPE),
     (dict(rot=24), SHAPE), (dict(rot=144), SHAPE), (dict(rot=-16), SHAPE), (dict(N=1), NULL),
     (dict(N=1, q=16, k=16, v=16, slots=16, q_out=16, rot=64), NULL),
-    (dict(N=1, q=24, k=16, v=16, slots=16, q_out=16), ALIGN), (dict(N=1, q=16, k=16, v=16, slots=16, q_out=16, k_norm=4), ALIGN),
+    (dict(N=1, q=24, k=16, v=16, slots=16, q_out=16), ALIGN), (dict(N=1, q=16, k=16, v=16, slots=16, q_out=16), ALIGN), (dict(N=1, q=16, k=16, v=16, slots=16, q_out=16, k_norm=4), ALIGN),
     (dict(N=1, q=16, k=16, v=16, slots=16, q_out=16, k_strides=(ctypes.c_int64 * 2)(0, 4)), ALIGN), (dict(), 0)])
 def test_c_abi_refuses_bad_appends(lib, bad, code):
     d = dict(struct_bytes=ctypes.sizeof(Append), cache=cache(), dtype=1, N=0, Hq=4)
@@ -166,7 +166,7 @@ def test_c_abi_refuses_bad_appends(lib, bad, code):
     assert status_of(lib.smb_kv_append, Append(**d)) == code
 
 
-READY = dict(N=1, q=16, out=16, kv_lens=16, q_starts=16, ws=16, block_table=16, max_pages=1)
+READY = dict(N=1, q=16, out=32, kv_lens=16, q_starts=16, ws=16, block_table=16, max_pages=1)
 
 
 @pytest.mark.parametrize("bad,code", [
@@ -174,7 +174,7 @@ READY = dict(N=1, q=16, out=16, kv_lens=16, q_starts=16, ws=16, block_table=16, 
     (dict(B=-1), SHAPE), (dict(N=1 << 30), SHAPE), (dict(scale=0.0), SHAPE), (dict(scale=-1.0), SHAPE),
     (dict(scale=float("nan")), SHAPE), (dict(scale=float("inf")), SHAPE), (dict(max_pages=-1), SHAPE),
     (dict(tree=16, tree_words=0), SHAPE), (dict(N=1), NULL), (dict(READY, block_table=None), NULL), (dict(READY, ws=None), NULL),
-    (dict(READY, q=8), ALIGN), (dict(READY, out=4), ALIGN), (dict(READY, q_strides=(ctypes.c_int64 * 2)(128, 20)), ALIGN),
+    (dict(READY, cache=cache(num_pages=0)), SHAPE), (dict(READY, out=16), ALIGN), (dict(READY, q=8), ALIGN), (dict(READY, out=4), ALIGN), (dict(READY, q_strides=(ctypes.c_int64 * 2)(128, 20)), ALIGN),
     (dict(B=0, N=1), 0), (dict(), 0)])
 def test_c_abi_refuses_bad_attention(lib, bad, code):
     d = dict(struct_bytes=ctypes.sizeof(Attention), cache=cache(), dtype=1, N=0, Hq=4, B=1, scale=1.0)
