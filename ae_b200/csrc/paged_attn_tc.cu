@@ -18,6 +18,13 @@
 //    the end.  Bound by memory at the sizes of a verify step: a 64 KB tile takes an SM's share of HBM
 //    about 2800 clocks, twice what its products and exponentials take.
 //
+// Measured (sustained, under the power cap): 16 sequences of up to 16384 keys, trees of 32 tokens, 48 / 8
+// heads of 128: 707 MB of cache and 109 GFLOP in 190-225 us (3.1-3.7 TB/s); two chunks of 2048 tokens
+// over 8191 keys: 290 GFLOP in 300-335 us (870-970 TFLOP/s).  A 128-key tile of a stream takes 3250
+// clocks: 250 to read S, 200 for the maximum, 1450 for the exponentials and P (1024 of them at best when
+// the other stream leaves the units alone), 1250 until the next S (256 for what is left of the second
+// product, 512 for the first, the rest in handovers and behind the other stream's products).
+//
 // Keys and values come by TMA, one box per page (its rows of one head) and 64 dims, into a ring of
 // five 128-row slots with the 128-byte swizzle.  Keys past the end and pages outside the cache are
 // boxes at a page coordinate past the tensor: TMA writes zeros there, and the mask drops them.  Rows
@@ -29,7 +36,8 @@
 // products with Q are done, so that a segment's first S is there when its predecessor's output has been
 // written.
 //
-// A 4-bit cache has four more warps in the place of TMA's K and V: rows come packed by cp.async into a
+// A 4-bit cache (32 / 8 heads, else as above: 224 MB in 205 us, bound by the unpacking, 2000 clocks for the
+// 128 rows of a slot) has four more warps in the place of TMA's K and V: rows come packed by cp.async into a
 // ring of each warp's own, and go as values of the 16-bit type into the slots (scale x code + zero,
 // one rounding: the score of a key is then off by at most half a step of each of its values, as if the
 // cache were of the 16-bit type; applying the scales to the products instead, as the kernel for few
@@ -935,10 +943,13 @@ bool tc_takes(const PagedCacheArgs& c, bool bits4) {
   return bits4 || (c.page_shift >= 3 && c.num_pages >= 1 && c.num_pages < 0x7fffffffll);
 }
 
-bool plan_attn_tc(int N, int B, int g, int D, int sms, AttnPlan* p) {
+// Two row tiles at a time where a key head has more than 128 rows: at 136 to 192 rows (16 sequences of
+// 8192 keys) 148-150 us against 197-205 with the keys read once per row tile (16 bits), 180-187 against
+// 290-302 (4 bits); at 128 rows 146 against 109-117.
+bool plan_attn_tc(int N, int B, int g, int D, bool bits4, int sms, AttnPlan* p) {
   if (D > 128 || g > 128) return false;
   const long long rows = (static_cast<long long>(N) * g + B - 1) / B;
-  if (rows <= kTcMinRows) return false;
+  if (rows <= (bits4 ? kTcAboveRows4 : kTcAboveRows16)) return false;
   p->rows = rows > 128 ? 256 : 128;
   p->grid = sms;
   p->min_tiles = 2;

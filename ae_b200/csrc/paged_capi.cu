@@ -151,7 +151,7 @@ size_t smb_paged_attention_workspace_bytes(int N, int B, int Hq, int Hkv, int he
   const int g = Hq / Hkv;
   size_t n = attn_ws(plan_attn_mma(N, B, g, head_dim, bits == 4, di.sms), head_dim);
   AttnPlan p;
-  if (plan_attn_tc(N, B, g, head_dim, di.sms, &p)) n = std::max(n, attn_ws(p, head_dim));
+  if (plan_attn_tc(N, B, g, head_dim, bits == 4, di.sms, &p)) n = std::max(n, attn_ws(p, head_dim));
   if (bits == 4 && plan_attn_q4(N, B, g, head_dim, di.sms, &p)) n = std::max(n, attn_ws(p, head_dim));
   return n;
 }
@@ -216,7 +216,7 @@ int smb_paged_attention(const smb_attention_args_t* r, smb_stream_t stream) {
     a.seg_cost = p.seg_cost;
     return r->ws_bytes >= attn_ws(p, D);
   };
-  if (tc_takes(a.c, bits4) && plan_attn_tc(N, B, a.g, D, di.sms, &p)) {
+  if (tc_takes(a.c, bits4) && plan_attn_tc(N, B, a.g, D, bits4, di.sms, &p)) {
     if (!use()) return SMB_ERR_WORKSPACE;
     bool fits = false;
     const cudaError_t err = launch_attn_tc(a, p, D, bf16, bits4, st, pdl_enabled(), &fits);
