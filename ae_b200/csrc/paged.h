@@ -97,7 +97,7 @@ struct AttnPlan {
 AttnPlan plan_attn_mma(int N, int B, int g, int D, bool bits4, int sms);
 cudaError_t launch_attn_mma(AttnArgs a, const AttnPlan& p, int D, bool bf16, bool bits4, cudaStream_t stream, bool pdl);
 // 4-bit caches and at most 8 query rows of a key head on average (false otherwise).  16 sequences of 8192
-// keys: 73 us at 8 rows, against 99 us of the kernel for 16.
+// keys, 8 key heads of 128: 72-74 us at 4 and 8 rows, 96-97 us by the kernel for 16 rows.
 bool plan_attn_q4(int N, int B, int g, int D, int sms, AttnPlan* p);
 cudaError_t launch_attn_q4(AttnArgs a, const AttnPlan& p, int D, bool bf16, cudaStream_t stream, bool pdl);
 // tcgen05 kernel: plan_attn_tc is false for few rows and heads of 256, tc_takes for 16-bit caches with
@@ -105,7 +105,7 @@ cudaError_t launch_attn_q4(AttnArgs a, const AttnPlan& p, int D, bool bf16, cuda
 // make a tensor map.
 // From how many query rows of a key head (on average over the sequences).  16 sequences of 8192 keys,
 // 8 key heads of 128, tcgen05 against the other kernel: 16 bits 106 / 97 us at 16 rows, 106 / 115 at 24
-// and 32, 107 / 199 at 48; 4 bits 165 / 154 us at 32 rows, 174 / 230 at 48.
+// and 32, 107 / 199 at 48; 4 bits 165 / 153 us at 32 rows, 174 / 230 at 48.
 constexpr int kTcAboveRows16 = 16, kTcAboveRows4 = 32;
 bool tc_takes(const PagedCacheArgs& c, bool bits4);
 bool plan_attn_tc(int N, int B, int g, int D, bool bits4, int sms, AttnPlan* p);

@@ -20,10 +20,9 @@
 //
 // Measured (sustained, under the power cap): 16 sequences of up to 16384 keys, trees of 32 tokens, 48 / 8
 // heads of 128: 707 MB of cache and 109 GFLOP in 190-225 us (3.1-3.7 TB/s); two chunks of 2048 tokens
-// over 8191 keys: 290 GFLOP in 300-335 us (870-970 TFLOP/s).  A 128-key tile of a stream takes 3250
-// clocks: 250 to read S, 200 for the maximum, 1450 for the exponentials and P (1024 of them at best when
-// the other stream leaves the units alone), 1250 until the next S (256 for what is left of the second
-// product, 512 for the first, the rest in handovers and behind the other stream's products).
+// over 8191 keys: 290 GFLOP in 295-370 us (785-985 TFLOP/s, with the SM clock).  A 128-key tile of a
+// stream takes about 3250 clocks (clock stamps): 280 to read S, 240 for the maximum, 1420 for the
+// exponentials and P, 1250 until the next S; the two streams' exponentials alone need 2048.
 //
 // Keys and values come by TMA, one box per page (its rows of one head) and 64 dims, into a ring of
 // five 128-row slots with the 128-byte swizzle.  Keys past the end and pages outside the cache are
@@ -36,7 +35,7 @@
 // products with Q are done, so that a segment's first S is there when its predecessor's output has been
 // written.
 //
-// A 4-bit cache (32 / 8 heads, else as above: 224 MB in 205 us, bound by the unpacking, 2000 clocks for the
+// A 4-bit cache (32 / 8 heads, else as above: 73 GFLOP in 205-216 us, bound by the unpacking, 2000 clocks for the
 // 128 rows of a slot) has four more warps in the place of TMA's K and V: rows come packed by cp.async into a
 // ring of each warp's own, and go as values of the 16-bit type into the slots (scale x code + zero,
 // one rounding: the score of a key is then off by at most half a step of each of its values, as if the
