@@ -11,6 +11,7 @@ namespace smb {
 
 constexpr int kPagedMaxHeads = 1024;  // query heads of one call
 constexpr int kPagedMaxPage = 65536;  // tokens of a page (a power of two)
+constexpr int kPagedMaxKeys = 1 << 30;  // that a row of the block table has pages for
 
 // Bytes of one row (a head of a token) of a 4-bit cache: D/2 bytes of codes, D/32 pairs of a
 // 16-bit scale and zero, rounded up to 16 bytes so that every row starts on 16 bytes.

@@ -167,6 +167,8 @@ int smb_paged_attention(const smb_attention_args_t* r, smb_stream_t stream) {
   rc = attn_sizes(N, B, r->Hq, a.c.Hkv, D, r->cache.bits);
   if (rc != SMB_OK) return rc;
   if (r->max_pages < 0 || r->table_stride < 0) return SMB_ERR_SHAPE;
+  // (the kernels count a sequence's keys, and the tile behind its last one, in 32 bits)
+  if (r->max_pages > kPagedMaxKeys >> a.c.page_shift) return SMB_ERR_SHAPE;
   if (r->tree != nullptr && (r->tree_words < 1 || r->tree_stride < 0)) return SMB_ERR_SHAPE;
   if (!(r->scale > 0.f) || r->scale > 1e30f) return SMB_ERR_SHAPE;
   if (N == 0 || B == 0) return SMB_OK;

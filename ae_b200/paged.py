@@ -310,6 +310,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.get_device() != dev:
         raise ValueError("block_table must be int32 [B, max_pages] on the device of q")
     B, max_pages = block_table.shape
+    if max_pages * cache[7] > 1 << 30:
+        raise ValueError(f"block_table has {max_pages} pages of {cache[7]} tokens for a sequence (at most 2^30 tokens)")
     table_stride, one = block_table.stride()
     if max_pages > 1 and one != 1:
         raise ValueError("a row of block_table must be contiguous")
@@ -331,6 +333,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     elif N > 0 and out.data_ptr() == q.data_ptr():
         raise ValueError("out may not be q")
     ots, ohs = _rows("out", out, shape, dtype, dev)
+    (inner, n), (outer, m) = sorted(((ots, N), (ohs, Hq)))
+    if (n > 1 and inner < D) or (m > 1 and outer < inner * (n - 1) + D):
+        raise ValueError("the rows of out may not overlap")
     if N > 0 and B > 0 and cache[2] == 0:
         raise ValueError("the cache has no pages")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (N, Hq) or lse.get_device() != dev

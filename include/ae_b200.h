@@ -428,6 +428,7 @@ SMB_API size_t smb_paged_attention_workspace_bytes(int N, int B, int Hq, int Hkv
  * trees: ancestors and itself; bits beyond the words read as 0).  out = softmax(scale * q k) v,
  * lse [N, Hq] (optional) = the natural log of the softmax's sum; a token that sees no key gets 0 and
  * -inf.  Rows of q that belong to no sequence leave out and lse as they were; out may not overlap q (SMB_ERR_ALIGN for q itself).
+ * max_pages * page_size may be 2^30 at most.
  * Lengths are read on the device: kv_lens is cut to max_pages * page_size, q_starts to [0, N]; keys of
  * a page outside [0, num_pages) are left out and recorded as 2 in *status (device int, optional).
  * (specmoe/layers/attention_backend/triton_backend.py, cpu_backend.py; the lse is what joins a

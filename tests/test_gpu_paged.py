@@ -578,6 +578,30 @@ def test_attention_option_refusals(kw):
         paged.paged_attention(**d)
 
 
+@pytest.mark.parametrize("strides,good", [((512, 128), True), ((128, 512), True), ((640, 136), True), ((0, 128), False),
+                                          ((128, 128), False), ((512, 0), False), ((256, 128), False), ((512, 64), False)])
+def test_rows_of_out_may_not_overlap(strides, good):
+    from ae_b200 import paged
+    d = make_batch([3, 1], [40, 7], 4, 2, 128, 16, BF, 16, False)
+    out = torch.zeros(4096, dtype=BF, device="cuda").as_strided((4, 4, 128), (*strides, 1))
+    if good:
+        assert torch.equal(paged.paged_attention(**d, out=out), paged.paged_attention(**d))
+    else:
+        with pytest.raises(ValueError, match="overlap"):
+            paged.paged_attention(**d, out=out)
+
+
+def test_tables_of_more_than_30_bits_are_refused():
+    from ae_b200 import paged
+    d = make_batch([1], [40], 4, 2, 64, 16, BF, 16, False)
+    d["k_cache"], d["v_cache"] = paged.new_cache(1, 2, 65536, 64, BF, "cuda")
+    d["block_table"] = torch.zeros(1, (1 << 14) + 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="2\\^30"):
+        paged.paged_attention(**d)
+    d["block_table"] = d["block_table"][:, :-1]
+    assert torch.isfinite(paged.paged_attention(**d)).all()
+
+
 @pytest.mark.parametrize("change", [
     dict(k=lambda c: c["k"][:, :1]), dict(v=lambda c: c["v"].float()), dict(slots=lambda c: c["slots"].int()),
     dict(slots=lambda c: c["slots"][:-1]), dict(positions=lambda c: c["positions"].int()),

@@ -182,6 +182,15 @@ def test_c_abi_refuses_bad_attention(lib, bad, code):
     assert status_of(lib.smb_paged_attention, Attention(**d)) == code
 
 
+@pytest.mark.parametrize("page_size,most", [(1, 1 << 30), (16, 1 << 26), (65536, 1 << 14)])
+def test_c_abi_refuses_tables_of_more_than_30_bits(lib, page_size, most):
+    """Key indexes, and the end of the tile behind the last key, are 32-bit integers."""
+    d = dict(struct_bytes=ctypes.sizeof(Attention), cache=cache(page_size=page_size), dtype=1, N=0, Hq=4, B=1, scale=1.0)
+    assert status_of(lib.smb_paged_attention, Attention(**d, max_pages=most)) == 0
+    assert status_of(lib.smb_paged_attention, Attention(**d, max_pages=most + 1)) == SHAPE
+    assert status_of(lib.smb_paged_attention, Attention(**d, max_pages=(1 << 31) - 1)) == SHAPE
+
+
 def test_c_abi_null_and_read(lib):
     assert lib.smb_kv_append(None, None) == NULL and lib.smb_paged_attention(None, None) == NULL
     assert lib.smb_kv4_read(None, 1, None, 1, None, None) == NULL
