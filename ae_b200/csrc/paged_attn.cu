@@ -30,7 +30,8 @@
 //
 // What is masked contributes nothing whatever it holds: rows past the keys and rows of bad pages
 // are zero-filled, and where a mask cuts a tile, non-finite values are taken out of the product
-// and added to the rows that do see them.
+// and added to the rows that do see them.  For a 4-bit group that means its unpacked values: they may
+// overflow the 16-bit type though scale and zero are finite.
 #include <algorithm>
 
 #include "common.cuh"
@@ -334,8 +335,7 @@ __global__ void __launch_bounds__(128, (MmaCfg<D, MT, BITS4>::CTAS > 2 && MT == 
           }
         } else {
           for (int i = lane; i < KS * G; i += 32) {
-            const uint32_t v = *reinterpret_cast<const uint32_t*>(vs + (i / G) * ROW + D / 2 + (i % G) * 4);
-            bad = bad || H::nonfinite(v & 0xffffu) || H::nonfinite(v >> 16);
+            bad = bad || group_overflows<T>(*reinterpret_cast<const uint32_t*>(vs + (i / G) * ROW + D / 2 + (i % G) * 4));
           }
         }
         if (__any_sync(0xffffffffu, bad)) {
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(128, (MmaCfg<D, MT, BITS4>::CTAS > 2 && MT == 
                     } else {
                       const int d = (2 * c4 + e) * (D / 8) + t2;
                       const uint32_t sz = *reinterpret_cast<const uint32_t*>(vs + kl * ROW + D / 2 + (d >> 5) * 4);
-                      v = H::lo(sz) + H::hi(sz);
+                      v = H::lo(value_of<T>((vs[kl * ROW + (d >> 1)] >> (4 * (d & 1))) & 15u, sz));
                     }
                     if (!isfinite(v)) O[mt][t2][hh * 2 + e] += v;
                   }
@@ -372,8 +372,9 @@ __global__ void __launch_bounds__(128, (MmaCfg<D, MT, BITS4>::CTAS > 2 && MT == 
             }
           } else {
             for (int i = lane; i < KS * G; i += 32) {
-              uint32_t* p = reinterpret_cast<uint32_t*>(vs + (i / G) * ROW + D / 2 + (i % G) * 4);
-              if (H::nonfinite(*p & 0xffffu) || H::nonfinite(*p >> 16)) *p = 0;
+              uint8_t* row = vs + (i / G) * ROW;
+              uint32_t* sz = reinterpret_cast<uint32_t*>(row + D / 2 + (i % G) * 4);
+              if (group_overflows<T>(*sz)) take_out_nonfinite<T>(reinterpret_cast<uint32_t*>(row + (i % G) * 16), sz);
             }
           }
           __syncwarp();

@@ -220,8 +220,7 @@ __global__ void __launch_bounds__(128, Q4Cfg<D>::CTAS) paged_attn_q4_kernel(cons
         // non-finite values behind the mask: to the rows that see them directly, out of the product
         bool bad = false;
         for (int i = lane; i < KS * G; i += 32) {
-          const uint32_t v = *reinterpret_cast<const uint32_t*>(vs + (i / G) * ROW + D / 2 + (i % G) * 4);
-          bad = bad || H::nonfinite(v & 0xffffu) || H::nonfinite(v >> 16);
+          bad = bad || group_overflows<T>(*reinterpret_cast<const uint32_t*>(vs + (i / G) * ROW + D / 2 + (i % G) * 4));
         }
         if (__any_sync(0xffffffffu, bad)) {
           for (int kl = 0; kl < KS; ++kl) {
@@ -234,16 +233,18 @@ __global__ void __launch_bounds__(128, Q4Cfg<D>::CTAS) paged_attn_q4_kernel(cons
               for (int t2 = 0; t2 < MTD; ++t2)
 #pragma unroll
                 for (int e = h; e < 4; e += 2) {
-                  const uint32_t sz = *reinterpret_cast<const uint32_t*>(vs + kl * ROW + D / 2 + (dim_of(t2, e) >> 5) * 4);
-                  const float v = H::lo(sz) + H::hi(sz);
+                  const int d = dim_of(t2, e);
+                  const uint32_t sz = *reinterpret_cast<const uint32_t*>(vs + kl * ROW + D / 2 + (d >> 5) * 4);
+                  const float v = H::lo(value_of<T>((vs[kl * ROW + (d >> 1)] >> (4 * (d & 1))) & 15u, sz));
                   if (!isfinite(v)) O[t2][e] += v;
                 }
             }
           }
           __syncwarp();
           for (int i = lane; i < KS * G; i += 32) {
-            uint32_t* p = reinterpret_cast<uint32_t*>(vs + (i / G) * ROW + D / 2 + (i % G) * 4);
-            if (H::nonfinite(*p & 0xffffu) || H::nonfinite(*p >> 16)) *p = 0;
+            uint8_t* row = vs + (i / G) * ROW;
+            uint32_t* sz = reinterpret_cast<uint32_t*>(row + D / 2 + (i % G) * 4);
+            if (group_overflows<T>(*sz)) take_out_nonfinite<T>(reinterpret_cast<uint32_t*>(row + (i % G) * 16), sz);
           }
           __syncwarp();
         }

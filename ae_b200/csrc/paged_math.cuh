@@ -103,6 +103,37 @@ __device__ __forceinline__ uint32_t nib(uint32_t w) {
   return (v & Half2<T>::kMask) | Half2<T>::kBase;
 }
 
+// The value of a code of a 4-bit group with the pair `sz` (scale, zero), as the products get it: the 16-bit
+// number (in the low half) nearest code * scale + zero, which may overflow though all three are finite.
+template <typename T>
+__device__ __forceinline__ uint32_t value_of(uint32_t code, uint32_t sz) {
+  const uint32_t v = Half2<T>::kBase | (code * 0x00010001u << Half2<T>::kUp);
+  return Half2<T>::dequant(v, __byte_perm(sz, sz, 0x1010), __byte_perm(sz, sz, 0x3232)) & 0xffffu;
+}
+
+// Whether some code of such a group has a value that is not finite.  Rounding keeps the order, so the two
+// ends tell (an infinite scale makes NaN of code 0).
+template <typename T>
+__device__ __forceinline__ bool group_overflows(uint32_t sz) {
+  return Half2<T>::nonfinite(value_of<T>(0, sz)) || Half2<T>::nonfinite(value_of<T>(15, sz));
+}
+
+// Takes those values out of a group, to where a weight of 0 makes 0 of them; its finite values stay.  (A code whose value
+// overflows goes to code 0, whose value is the zero: the rows that see it are infinite there already.)
+template <typename T>
+__device__ __forceinline__ void take_out_nonfinite(uint32_t* codes, uint32_t* sz) {
+  const uint32_t pair = *sz;
+  if (Half2<T>::nonfinite(pair & 0xffffu) || Half2<T>::nonfinite(pair >> 16)) {
+    *sz = 0;
+    return;
+  }
+#pragma unroll 1
+  for (int e = 0; e < 32; ++e) {
+    const int sh = 4 * (e & 7);
+    if (Half2<T>::nonfinite(value_of<T>((codes[e >> 3] >> sh) & 15u, pair))) codes[e >> 3] &= ~(15u << sh);
+  }
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool fill) {
   const int n = fill ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");

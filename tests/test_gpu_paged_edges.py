@@ -1,0 +1,81 @@
+"""Paged cache and attention at the edges of the number formats (ae_b200/paged.py): values of a 4-bit
+cache that overflow the 16-bit type.
+
+A value of a 4-bit cache enters attention's second product as the 16-bit number nearest scale * code + zero.
+Both numbers of a group can be finite and that one not (fp16: 15 * 4368 = 65520 rounds to infinity).  A row that may
+not see such a value keeps its result bit for bit; a row that sees it gets that infinity (or NaN) in those
+dims, and everywhere else the tolerance of ``tests/test_gpu_paged.py``, derived there."""
+import math
+
+import pytest
+import torch
+
+from tests import paged_reference as ref
+from tests.test_gpu_paged import BF, FP, call, make_batch
+
+pytestmark = pytest.mark.gpu
+
+# Query heads over 2 key heads, 9 new tokens of 2 sequences: 5, 9, 18, 72 and 288 query rows of a key head on
+# average, which go to the kernels for up to 8, 16 and 32 rows and to the tensor cores' with one and two row
+# tiles at a time (heads of 256: to the first two).
+HEADS = [2, 4, 8, 32, 128]
+# scale and zero of a group as fractions of the largest finite number: code 15 overflows (in fp16 the scale that
+# rounding gives the group 0 to 65504; bf16's rounding keeps that one finite), all but code 0, the negative side,
+# and an infinite scale (code 0 is then NaN)
+GROUPS = {"upper": (4368 / 65504, 0.0), "upper bf16": (0.0675, 0.0), "all": (4368 / 65504, 1.0), "lower": (-4368 / 65504, -0.5), "scale": (math.inf, 0.0)}
+
+
+def masked_batch(heads, D, dtype, tree):
+    """The batch of ``test_masked_places_may_hold_anything``; the rows that see the newest token but one of
+    sequence 0."""
+    d = make_batch([6, 3], [70, 35], heads, 2, D, 16, dtype, 4, tree, seed=11)
+    if tree:
+        d["tree"] = torch.tensor([1, 3, 5, 9, 17, 33, 1, 3, 7], dtype=torch.int32, device="cuda")[:, None].contiguous()
+    return d, ([4] if tree else [4, 5])
+
+
+def spoil(d, D, dtype, scale, zero):
+    """Gives that token's values a second group of ``scale`` and ``zero`` with codes 0 to 15 in turn; returns its
+    32 values as 16-bit numbers."""
+    j = 70 - 2
+    row = d["v_cache"][int(d["block_table"][0, j // 16]), :, j % 16]
+    codes = torch.arange(32, device="cuda") % 16
+    row[:, 16:32] = (codes[0::2] + 16 * codes[1::2]).to(torch.uint8)
+    sz = torch.tensor([scale, zero], device="cuda", dtype=torch.float64).to(dtype)
+    row[:, D // 2 + 4:D // 2 + 8] = sz.view(torch.uint8)
+    return (codes.double() * sz[0].double() + sz[1].double()).to(dtype)
+
+
+@pytest.mark.parametrize("tree", [False, True], ids=["causal", "tree"])
+@pytest.mark.parametrize("dtype,kind", [(t, k) for t in (FP, BF) for k in GROUPS
+                                        if k != ("upper bf16" if t == FP else "upper")])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("heads", HEADS)
+def test_values_that_overflow_stay_behind_the_mask(heads, D, dtype, kind, tree):
+    d, sees = masked_batch(heads, D, dtype, tree)
+    good, good_lse = call(d)
+    most = torch.finfo(dtype).max
+    v16 = spoil(d, D, dtype, *(x * most for x in GROUPS[kind]))
+    over = ~torch.isfinite(v16)
+    assert bool(over.any()) and (kind == "scale") == bool(over.all())
+    out, lse = call(d)
+    assert torch.equal(lse, good_lse)  # keys are as they were
+    for i in range(9):
+        if i not in sees:
+            assert torch.equal(out[i], good[i]), i
+            continue
+        got = out[i, :, 32:64]
+        want = v16[over].double().expand(heads, -1)
+        assert torch.equal(torch.nan_to_num(got[:, over].double(), nan=7.0), torch.nan_to_num(want, nan=7.0)), i
+        assert torch.equal(out[i, :, :32], good[i, :, :32]) and torch.equal(out[i, :, 64:], good[i, :, 64:]), i
+    if dtype == FP and kind in ("upper", "lower"):  # (sums of bf16's largest numbers pass 32 bits)
+        # the finite neighbours in the group
+        o, _, spread, reach = ref.attention(d["q"], d["k_cache"], d["v_cache"], d["block_table"], d["kv_lens"],
+                                            d["q_starts"], d["tree"])
+        u = ref.half_step(dtype)
+        off = u * reach[..., None] if heads >= 32 and D <= 128 else torch.zeros_like(reach)[..., None]
+        tol = u * o.abs() + (2 * u + 2 ** -14 + torch.expm1(2 * off)) * spread + 2 ** -25
+        dims = 32 + torch.nonzero(~over)[:, 0]
+        for i in sees:
+            err = (out[i][:, dims].double() - o[i][:, dims]).abs()
+            assert bool((err <= tol[i][:, dims]).all()), i
