@@ -21,7 +21,8 @@
 //
 // A 4-bit row keeps, for each 32 values, zero = rn(min), scale = rn((max - min) / 15) in the
 // 16-bit type and codes rint((x - zero) / scale) in [0, 15]; the codes are formed with the
-// rounded scale and zero, so their rounding is not added to the codes' own.
+// rounded scale and zero, so their rounding is not added to the codes' own.  A group with a NaN has
+// both NaN, one with an infinity an infinite scale and codes of 0: either way it reads as NaN.
 #include <algorithm>
 #include <type_traits>
 
@@ -49,6 +50,18 @@ __device__ __forceinline__ uint64_t wide(uint32_t v) {
 __device__ __forceinline__ uint4 swap_pairs(uint4 v) {
   return make_uint4(__byte_perm(v.x, 0, 0x1032), __byte_perm(v.y, 0, 0x1032), __byte_perm(v.z, 0, 0x1032),
                     __byte_perm(v.w, 0, 0x1032));
+}
+
+// Minimum and maximum that are NaN if one of the two is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 constexpr int kAppendWarps = 4;   // of a CTA
@@ -220,13 +233,13 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 8) kv_append_kernel(const _
         float mn = v[0], mx = v[0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) {
-          mn = fminf(mn, v[e]);
-          mx = fmaxf(mx, v[e]);
+          mn = min_nan(mn, v[e]);
+          mx = max_nan(mx, v[e]);
         }
 #pragma unroll
         for (int s = 1; s < 4; s <<= 1) {
-          mn = fminf(mn, __shfl_xor_sync(kAll, mn, s));
-          mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, s));
+          mn = min_nan(mn, __shfl_xor_sync(kAll, mn, s));
+          mx = max_nan(mx, __shfl_xor_sync(kAll, mx, s));
         }
         const uint32_t sz = Half2<T>::pack(__fdiv_rn(mx - mn, 15.0f), mn);
         const float scale = Half2<T>::lo(sz), zero = Half2<T>::hi(sz);

@@ -1,4 +1,4 @@
-"""Paged cache and attention at the edges of the number formats (ae_b200/paged.py): values of a 4-bit
+"""Paged cache and attention at the edges of the number formats (ae_b200/paged.py): non-finite values, and values of a 4-bit
 cache that overflow the 16-bit type.
 
 A value of a 4-bit cache enters attention's second product as the 16-bit number nearest scale * code + zero.
@@ -79,3 +79,30 @@ def test_values_that_overflow_stay_behind_the_mask(heads, D, dtype, kind, tree):
         for i in sees:
             err = (out[i][:, dims].double() - o[i][:, dims]).abs()
             assert bool((err <= tol[i][:, dims]).all()), i
+
+
+def append_values(v):
+    """v [N, 1, D] appended as keys and as values of a 4-bit cache: both read back."""
+    from ae_b200 import paged
+    N, _, D = v.shape
+    kc, vc = paged.new_cache(N // 16 + 1, 1, 16, D, v.dtype, "cuda", bits=4)
+    slots = torch.arange(N, device="cuda")
+    paged.kv_append(v.clone(), v, v, kc, vc, slots)
+    return [paged.kv4_read(c, slots, D, v.dtype) for c in (kc, vc)]
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", [FP, BF], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_nonfinite_values_are_not_lost_in_4_bits(D, dtype, value):
+    """A NaN or an infinity among keys or values makes its group of 32 NaN, wherever in the group it is, and no other."""
+    G = D // 32
+    v = torch.randn(32 * G, 1, G, 32, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda").to(dtype)
+    row = torch.arange(32 * G, device="cuda")
+    want = torch.zeros(32 * G, 1, G, dtype=torch.bool, device="cuda")
+    clean = append_values(v.view(-1, 1, D))
+    v[row, 0, row // 32, row % 32] = value
+    want[row, 0, row // 32] = True
+    for got, was in zip(append_values(v.view(-1, 1, D)), clean):
+        assert bool(torch.isnan(got.view_as(v)[want]).all())
+        assert torch.equal(got.view_as(v)[~want], was.view_as(v)[~want])
