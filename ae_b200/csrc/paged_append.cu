@@ -20,7 +20,7 @@
 // copy rate; issue slots 75 % busy).
 //
 // A 4-bit row keeps, for each 32 values, zero = rn(min), scale = rn((max - min) / 15) in the
-// 16-bit type and codes rint((x - zero) / scale) in [0, 15]; the codes are formed with the
+// 16-bit type (rounded down if 15 scale + zero would overflow it: 0 to 65504 in fp16) and codes rint((x - zero) / scale) in [0, 15]; the codes are formed with the
 // rounded scale and zero, so their rounding is not added to the codes' own.  A group with a NaN has
 // both NaN, one with an infinity an infinite scale and codes of 0: either way it reads as NaN.
 #include <algorithm>
@@ -62,6 +62,18 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+
+// The (scale, zero) of a 4-bit group whose smallest and largest values are mn and mx, with the scale taken down
+// where needed for code 15 to stay finite; as it is where mx or the zero does not fit the type.
+template <typename T>
+__device__ __forceinline__ uint32_t fit_scale(uint32_t sz, float mn, float mx) {
+  using H = Half2<T>;
+  if (H::nonfinite(H::pack(mx, 0.f) & 0xffffu) || H::nonfinite(sz >> 16)) return sz;
+  const uint32_t zero = sz & 0xffff0000u;
+  if (H::nonfinite(sz & 0xffffu)) sz = zero | (H::pack(mx / 15.f - mn / 15.f, 0.f) & 0xffffu);  // (the span itself did)
+  if (group_overflows<T>(sz)) sz = zero | H::towards_zero(H::kMost / 15.f - H::hi(zero) / 15.f);
+  return sz;
 }
 
 constexpr int kAppendWarps = 4;   // of a CTA
@@ -241,8 +253,17 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 8) kv_append_kernel(const _
           mn = min_nan(mn, __shfl_xor_sync(kAll, mn, s));
           mx = max_nan(mx, __shfl_xor_sync(kAll, mx, s));
         }
-        const uint32_t sz = Half2<T>::pack(__fdiv_rn(mx - mn, 15.0f), mn);
-        const float scale = Half2<T>::lo(sz), zero = Half2<T>::hi(sz);
+        const float span = mx - mn;
+        uint32_t sz = Half2<T>::pack(__fdiv_rn(span, 15.0f), mn);
+        float scale = Half2<T>::lo(sz), zero = Half2<T>::hi(sz);
+        // (below 0.98 of the largest number no rounding of scale and zero takes code 15 past it)
+        if (fmaxf(mx, span) > 0.98f * Half2<T>::kMost) {
+          sz = fit_scale<T>(sz, mn, mx);
+          const float down = span > 3.3e38f ? 0.25f : 1.f;  // (v - zero may pass 32 bits: a quarter of everything)
+          scale = Half2<T>::lo(sz) * down, zero = Half2<T>::hi(sz) * down;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= down;
+        }
         // (a group of one value, or with a scale below the type, has codes of 0)
         const float inv = scale > 0.f ? __frcp_rn(scale) : 0.f;
         uint32_t codes = 0;

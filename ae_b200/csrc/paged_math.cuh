@@ -55,6 +55,8 @@ struct Half2<__nv_bfloat16> {
   // 16 + nibble e (and e + 4) of w: ulp of 16.0 is 2^-3, so the nibble goes to mantissa bits 3-6
   static constexpr uint32_t kMask = 0x00780078u, kBase = 0x41804180u;
   static constexpr int kUp = 3;
+  static constexpr float kMost = 3.38953138925153547590e38f;  // the largest finite number
+  static __device__ __forceinline__ uint32_t towards_zero(float x) { return __bfloat16_as_ushort(__float2bfloat16_rz(x)); }
   static __device__ __forceinline__ uint32_t dequant(uint32_t v, uint32_t s2, uint32_t z2) {
     const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&v);
     const uint32_t base = kBase;
@@ -80,6 +82,8 @@ struct Half2<__half> {
   // ulp of 16.0 is 2^-6: mantissa bits 6-9
   static constexpr uint32_t kMask = 0x03C003C0u, kBase = 0x4C004C00u;
   static constexpr int kUp = 6;
+  static constexpr float kMost = 65504.f;  // the largest finite number
+  static __device__ __forceinline__ uint32_t towards_zero(float x) { return __half_as_ushort(__float2half_rz(x)); }
   static __device__ __forceinline__ uint32_t dequant(uint32_t v, uint32_t s2, uint32_t z2) {
     const __half2 x = *reinterpret_cast<const __half2*>(&v);
     const uint32_t base = kBase;

@@ -224,9 +224,9 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
     a call have to be distinct.  ``positions`` int64 [N] and ``inv_freq`` float64 [rot / 2]
     (:func:`rope_inv_freq`) rotate the first ``rot`` dims: pairs (i, i + rot/2), or (2i, 2i + 1) when
     ``interleaved``; both None: no rotation.  ``q_norm`` / ``k_norm`` [head_dim]: weights of an RMS norm
-    of each head before the rotation.  In a 4-bit cache a group of 32 dims with a NaN or an infinity
-    among them reads as NaN.  ``status`` int32 [1], set to :data:`BAD_PAGE` by a slot past
-    the cache (which is not written)."""
+    of each head before the rotation.  Values that fit the type stay finite in a 4-bit cache; a group
+    of 32 dims with a NaN or an infinity among them reads as NaN.  ``status`` int32 [1], set to
+    :data:`BAD_PAGE` by a slot past the cache (which is not written)."""
     dev, dtype, code, shape = _query(q)
     N, Hq, D = shape
     cache = _cache(k_cache, v_cache, D, dtype, dev)

@@ -372,7 +372,9 @@ SMB_API int smb_moe_read_timers(const void* ws, size_t ws_bytes, int reset, smb_
  * place.  bits = 16: a row is head_dim values of `dtype`.  bits = 4: a row is
  * smb_kv4_row_bytes(head_dim) bytes: head_dim / 2 bytes of codes (dim 2i in the low nibble of
  * byte i), then a (scale, zero) pair of `dtype` for each 32 dims, then padding to 16 bytes;
- * a value is scale * code + zero.  (A group that was appended with a NaN or an infinity in it reads as NaN.)
+ * a value is scale * code + zero.  smb_kv_append takes zero = rn(min) and scale =
+ * rn((max - min) / 15), rounded down where 15 * scale + zero would overflow the type; a group with a NaN or an
+ * infinity in it reads as NaN.
  * Limits: head_dim 64, 128 or 256; page_size a power of two up to 65536; query heads a multiple
  * of kv_heads, at most 1024; tokens x query heads below 2^31; tensors 16-byte aligned. */
 typedef struct smb_paged_cache {

@@ -106,3 +106,33 @@ def test_nonfinite_values_are_not_lost_in_4_bits(D, dtype, value):
     for got, was in zip(append_values(v.view(-1, 1, D)), clean):
         assert bool(torch.isnan(got.view_as(v)[want]).all())
         assert torch.equal(got.view_as(v)[~want], was.view_as(v)[~want])
+
+
+@pytest.mark.parametrize("dtype", [FP, BF], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_values_that_fit_the_type_are_read_back_finite(D, dtype):
+    """Groups that reach the largest finite number, from any smallest one (their span passes 32 bits in bf16).
+
+    The scale is rounded to the type (u), or taken down to the largest one for which code 15 fits (2 u of the
+    largest number less the zero, for code 15 to fall short), the zero is rounded (u |lo|), half a step for
+    the code, and kv4_read rounds once (u |v|)."""
+    most = torch.finfo(dtype).max
+    g = torch.Generator(device="cuda").manual_seed(3)
+    N = 512
+    lo = torch.rand(N, 1, D // 32, 1, generator=g, device="cuda", dtype=torch.float64) * 2 - 1
+    lo[::7] = -1.0
+    lo[1::7] = 0.0
+    hi = torch.ones_like(lo)
+    hi[2::7] = 1 - 0.02 * torch.rand(hi[2::7].shape, generator=g, device="cuda", dtype=torch.float64)
+    x = lo + (hi - lo) * torch.rand(N, 1, D // 32, 32, generator=g, device="cuda", dtype=torch.float64)
+    x[..., 5:6], x[..., 9:10] = lo, hi
+    v = (x * most).to(dtype)
+    assert bool(torch.isfinite(v).all())
+    v64 = v.double()
+    lo, hi = v64.amin(-1, keepdim=True), v64.amax(-1, keepdim=True)
+    u = ref.half_step(dtype)
+    tol = (hi - lo) / 30 * (1 + 2 * u) + 2 * u * (most - lo) + u * lo.abs() + u * v64.abs()
+    for got in append_values(v.view(N, 1, D)):
+        assert bool(torch.isfinite(got).all())
+        err = (got.double().view_as(v64) - v64).abs()
+        assert bool((err <= tol * (1 + 2 ** -20)).all()), float((err / tol).max())
