@@ -216,8 +216,8 @@ __global__ void __launch_bounds__(BITS4 ? kTThreads4 : kTThreads, 1)
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* sm = dyn_smem + (base - raw);
   const uint32_t q_s = base, ring_s = base + C::Q;
-  // the plan lies where the ring will be: the first copy into it follows the first segment, and that
-  // follows the last look at the plan
+  // the plan lies where the ring will be: every thread but warp 3's is done with it at the barrier behind
+  // plan_build, and warp 3 before it hands out the first segment, which the first copy into the ring follows
   PlanShared* plan = reinterpret_cast<PlanShared*>(sm + C::Q);
 
   if (tid == 0) {
@@ -259,6 +259,8 @@ __global__ void __launch_bounds__(BITS4 ? kTThreads4 : kTThreads, 1)
   pdl_launch_dependents();
   const int cta = blockIdx.x;
   const long long W = plan_build<kTBK>(a, plan, gridDim.x);
+  fence_async_proxy();  // (TMA writes there next)
+  __syncthreads();
   int* status = a.status;
   volatile int* abort_flag = &s_abort;
 
@@ -340,6 +342,7 @@ __global__ void __launch_bounds__(BITS4 ? kTThreads4 : kTThreads, 1)
         // ---------------------------------------------------------------- segments
         Work k;
         bool more = work_begin<kTBK>(a, plan, W, cta, gridDim.x, k);
+        fence_async_proxy();
         __syncwarp();  // (the first segment gives the plan's place to the ring: every lane has read it)
         if (!more && lane == 0) leave_record(a, cta, k);
         while (more) {
