@@ -623,7 +623,9 @@ __global__ void __launch_bounds__(BITS4 ? kTThreads4 : kTThreads, 1)
           const bool cut = j0 + kTBK > g.open || j0 + kTBK > g.keys;
           mbar_wait(&s_bar[s], ns & 1, status, abort_flag);
           tc_fence_after();
-          if (cut) {
+          // (with two row tiles over the same V the first stream looks after it for both: a thread fences its own
+          // stores, and the second stream's product is issued behind the first one's)
+          if (cut && (!DUAL || s == 0)) {
             // V: what no mask stops from entering the product has to be finite.  (S being there says that
             // what its slot held before has been used, so that the wait can only be for this V.)
             const int vstep = it + (DUAL ? 2 * i + 1 : i + min(i + 2, n));

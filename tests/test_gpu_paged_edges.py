@@ -136,3 +136,29 @@ def test_values_that_fit_the_type_are_read_back_finite(D, dtype):
         assert bool(torch.isfinite(got).all())
         err = (got.double().view_as(v64) - v64).abs()
         assert bool((err <= tol * (1 + 2 ** -20)).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("heads", [8, 32])
+def test_nonfinite_values_in_every_masked_tile_again_and_again(heads, bits):
+    """A tree of 300 tokens, two row tiles or more over the same masked tiles, in which each 13th token has NaN or
+    infinite values and is seen by itself alone: the other rows are as they were, each time."""
+    d = make_batch([300], [430], heads, 2, 128, 16, BF, bits, True, seed=12)
+    bad = torch.arange(300, device="cuda") % 13 == 7
+    words = d["tree"]
+    for i in torch.nonzero(bad)[:, 0].tolist():
+        bit = (1 << (i % 32)) - (1 << 32 if i % 32 == 31 else 0)
+        words[:, i // 32] &= ~bit
+        words[i, i // 32] |= bit
+    good, good_lse = call(d)
+    for i in torch.nonzero(bad)[:, 0].tolist():
+        row = d["v_cache"][int(d["block_table"][0, (130 + i) // 16]), :, (130 + i) % 16]
+        value = (math.nan, math.inf, -math.inf)[i % 3]
+        if bits == 16:
+            row[:] = value
+        else:
+            row[:, 64:80] = torch.tensor([1.0, value] * 4, dtype=BF, device="cuda").view(torch.uint8)
+    for _ in range(30):
+        out, lse = call(d)
+        assert torch.equal(lse, good_lse) and torch.equal(out[~bad], good[~bad])
+        assert not bool(torch.isfinite(out[bad]).any())
