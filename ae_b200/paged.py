@@ -25,6 +25,7 @@ import functools
 import math
 from typing import List, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
 from . import _native, ops
@@ -166,6 +167,31 @@ def _rows(name: str, t: torch.Tensor, shape, dtype: torch.dtype, dev: int):
     return ts, hs
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two sets of rows [n, heads, head_dim] (rows contiguous, one dtype) share an element."""
+    D = a.shape[2]
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    levels = [sorted(((s, n) for s, n in zip(t.stride(), t.shape[:2]) if n > 1), reverse=True) for t in (a, b)]
+    pa, pb = (t.data_ptr() // t.element_size() for t in (a, b))
+
+    def span(lv):
+        return sum(s * (n - 1) for s, n in lv) + D
+
+    if pa + span(levels[0]) <= pb or pb + span(levels[1]) <= pa:
+        return False
+    if levels[0] and levels[1] and levels[0][0][0] == levels[1][0][0] > 0:
+        # slices of one buffer: side by side within its outer stride
+        period, ea, eb = levels[0][0][0], span(levels[0][1:]), span(levels[1][1:])
+        if ea <= (pb - pa) % period <= period - eb:
+            return False
+    starts = [np.sort(np.add.outer(np.arange(t.shape[0]) * t.stride(0), np.arange(t.shape[1]) * t.stride(1)).ravel() + p)
+              for t, p in ((a, pa), (b, pb))]
+    after = np.searchsorted(starts[1], starts[0] - D, side="right")  # the first row of b that ends behind a's start
+    near = after < starts[1].size
+    return bool((starts[1][after[near]] < starts[0][near] + D).any())
+
+
 def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, n: int, dev: int) -> int:
     if t.dtype != dtype or t.shape != (n,) or t.get_device() != dev or (n > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} must be contiguous {dtype} [{n}] on the device of q")
@@ -217,7 +243,7 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
               q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
               out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotate the new tokens' queries and keys and write keys and values into the cache; returns the
-    queries ``[N, Hq, head_dim]`` (``out``, contiguous, if given; it may not overlap q).
+    queries ``[N, Hq, head_dim]`` (``out``, contiguous, if given; it may not overlap q, k or v).
 
     q ``[N, Hq, head_dim]``, k and v ``[N, kv_heads, head_dim]`` (views of the projection's output are
     taken as they are).  ``slots`` int64 [N]: where each token goes; negative: nowhere.  The slots of
@@ -248,8 +274,12 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
         out = q.new_empty(shape)
     elif out.shape != shape or out.dtype != dtype or out.get_device() != dev or not out.is_contiguous():
         raise ValueError("out must be contiguous, with the shape, dtype and device of q")
-    elif N > 0 and out.data_ptr() == q.data_ptr():
-        raise ValueError("out may not be q")
+    else:
+        for name, t in (("q", q), ("k", k), ("v", v)):
+            if _overlap(out, t):
+                raise ValueError(f"out may not overlap {name}")
+    if N > 0 and cache[2] > 0 and cache[0] == cache[1]:
+        raise ValueError("k_cache and v_cache may not be the same array")
     word, mine = _status_word(status, dev)
     args = _native.APPEND_ARGS
     rc = _launch(dev, _native.load().smb_kv_append, args.pack(
@@ -329,14 +359,15 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         tree_p = tree.data_ptr()
         if N == 0:
             tree_p = 0
-    if out is None:
+    given = out is not None
+    if not given:
         out = q.new_empty(shape)
-    elif N > 0 and out.data_ptr() == q.data_ptr():
-        raise ValueError("out may not be q")
     ots, ohs = _rows("out", out, shape, dtype, dev)
     (inner, n), (outer, m) = sorted(((ots, N), (ohs, Hq)))
     if (n > 1 and inner < D) or (m > 1 and outer < inner * (n - 1) + D):
         raise ValueError("the rows of out may not overlap")
+    if given and _overlap(out, q):
+        raise ValueError("out may not overlap q")
     if N > 0 and B > 0 and cache[2] == 0:
         raise ValueError("the cache has no pages")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (N, Hq) or lse.get_device() != dev
