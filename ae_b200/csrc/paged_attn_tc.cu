@@ -45,7 +45,8 @@
 // when they are stored.
 //
 // Every wait is bounded, and no role waits at a hardware barrier inside its loop: after a failed wait
-// each role runs out of segments by itself (the results are void, the status says so).
+// each role runs out of segments by itself (the results are void; the caller's status word, if there is
+// one, says so).
 #include <algorithm>
 #include <type_traits>
 

@@ -218,14 +218,26 @@ def _status_word(status: Optional[torch.Tensor], dev: int):
     return None, False
 
 
-#: Device code that ``status`` gets for a page or slot outside the cache.
+#: Device codes that ``status`` gets (the first one stays): a page or slot outside the cache, which was left
+#: out, and a device wait of :func:`paged_attention` that ran past its limit, after which the call's results are
+#: void.  Without a ``status`` of the caller's, and without ``SMB_DEBUG=1``, neither is recorded anywhere.
 BAD_PAGE = 2
+TIMEOUT = 1
 
 
 def _raise_status(name: str, status: torch.Tensor):
     code = int(status.item())
     if code != 0:
         _native.check(name + " (device status)", -10 if code == BAD_PAGE else -9)
+
+
+def check_status(status: torch.Tensor):
+    """Reads (synchronously) and clears the ``status`` word of earlier calls; raises what it holds."""
+    try:
+        _raise_status("paged cache", status)
+    except _native.NativeError:
+        status.zero_()
+        raise
 
 
 def _query(q: torch.Tensor):
@@ -331,7 +343,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     optional: receives the natural log of each softmax's sum (-inf, with an output of 0, for a token
     that sees no key).  Rows of q behind the last sequence leave ``out`` and ``lse`` as they were.
     ``out`` may not overlap q.  ``status`` int32 [1] is set to :data:`BAD_PAGE` by a page outside the
-    cache (its keys are left out)."""
+    cache (its keys are left out), to :data:`TIMEOUT` by a call whose results are void;
+    :func:`check_status` reads it."""
     dev, dtype, code, shape = _query(q)
     N, Hq, D = shape
     cache = _cache(k_cache, v_cache, D, dtype, dev)

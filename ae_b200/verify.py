@@ -96,7 +96,9 @@ class VerifyDecoder:
     layer on the device: ``pools[l]`` [E, 3*I*H], page table identity.
 
     ``cache``: "dense", "paged" or "paged4", with pages of ``page_size`` tokens; the same seed
-    gives the same weights and cached values for each (rounded to 4 bits by the last)."""
+    gives the same weights and cached values for each (rounded to 4 bits by the last).  The paged calls of all
+    layers share the device word ``status``; :meth:`check_status` after a step, where its tokens are read
+    back, raises what they recorded."""
 
     def __init__(self, cfg: DecoderConfig, batch: int, cache_len: int, max_draft: int, device,
                  dtype=torch.bfloat16, seed: int = 0, moe: Optional[Callable] = None, cache: str = "dense",
@@ -148,6 +150,7 @@ class VerifyDecoder:
         places = torch.arange(per * page_size, device=self.device)
         self.slots = (self.block_table.long()[:, places // page_size] * page_size + places % page_size)  # [B, places]
         self.inv_freq, _ = paged.rope_inv_freq(c.head_dim, c.rope_theta, device=self.device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         for li in range(c.layers):
             k, v = (t.transpose(1, 2)[:, :n].reshape(B * n, c.kv_heads, c.head_dim).contiguous()
                     for t in (self.k_cache[li], self.v_cache[li]))
@@ -163,9 +166,16 @@ class VerifyDecoder:
         x = (h @ L["wqkv"].t()).view(B * n, c.heads + 2 * c.kv_heads, c.head_dim)
         q, k, v = x[:, :c.heads], x[:, c.heads:c.heads + c.kv_heads], x[:, c.heads + c.kv_heads:]
         kc, vc = self.k_cache[layer], self.v_cache[layer]
-        q = paged.kv_append(q, k, v, kc, vc, step["slots"], step["positions"], self.inv_freq)
-        o = paged.paged_attention(q, kc, vc, self.block_table, step["kv_lens"], step["q_starts"], tree=step["tree"])
+        status = None if ops.DEBUG else self.status  # (SMB_DEBUG=1: every call reads a word of its own)
+        q = paged.kv_append(q, k, v, kc, vc, step["slots"], step["positions"], self.inv_freq, status=status)
+        o = paged.paged_attention(q, kc, vc, self.block_table, step["kv_lens"], step["q_starts"], tree=step["tree"],
+                                  status=status)
         return o.view(B, n, c.heads * c.head_dim) @ L["wo"].t()
+
+    def check_status(self):
+        """Raises if a page or slot lay outside the cache, or a device wait ran out, since the last check."""
+        if self.cache != "dense":
+            paged.check_status(self.status)
 
     def _paged_step(self, parents: List[int]) -> dict:
         """What the layers of one step share: slots, positions, lengths and the trees' words."""

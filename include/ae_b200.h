@@ -395,7 +395,7 @@ SMB_API int smb_kv4_row_bytes(int head_dim);
  * q_out [N, Hq, head_dim] and keys and values to the rows of slots[t] (specmoe/models/mixtral.py:
  * 118-224 rotates and caches in separate kernels).  Strides {token, head} in elements, multiples of
  * 8; head_dim is contiguous.  A negative slot is not written; a slot past the cache is not written
- * and recorded as 2 in *status (device int, NULL: not recorded).  The slots of a call have to be
+ * and recorded as 2 in *status (device int, set to 0 by the caller; NULL: not recorded).  The slots of a call have to be
  * distinct; q_out may not overlap q. */
 typedef struct smb_append_args {
   size_t struct_bytes; /* sizeof(smb_append_args_t) */
@@ -432,7 +432,9 @@ SMB_API size_t smb_paged_attention_workspace_bytes(int N, int B, int Hq, int Hkv
  * -inf.  Rows of q that belong to no sequence leave out and lse as they were; out may not overlap q (SMB_ERR_ALIGN for q itself).
  * max_pages * page_size may be 2^30 at most.
  * Lengths are read on the device: kv_lens is cut to max_pages * page_size, q_starts to [0, N]; keys of
- * a page outside [0, num_pages) are left out and recorded as 2 in *status (device int, optional).
+ * a page outside [0, num_pages) are left out and recorded as 2 in *status (device int, optional).  A device
+ * wait that ran past its limit (2 s) is recorded there as 1, and the call's results are void; the first code
+ * stays, and without a status neither is recorded.
  * (specmoe/layers/attention_backend/triton_backend.py, cpu_backend.py; the lse is what joins a
  * result with another part of the context, as the reference joins its CPU and GPU parts.) */
 typedef struct smb_attention_args {
