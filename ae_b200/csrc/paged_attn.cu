@@ -388,8 +388,7 @@ __global__ void __launch_bounds__(128, (MmaCfg<D, MT, BITS4>::CTAS > 2 && MT == 
             for (int e = 0; e < 4; ++e) S[mt][n][e] *= a.scale_log2;
       }
 
-      // running maximum: a row's output is rescaled only when its maximum grew by more than 8 (a
-      // factor of 256; p then stays below 2^8, inside both 16-bit types), so most tiles skip it
+      // running maximum (paged_math.cuh)
       uint32_t P[MT][KS / 16][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -405,11 +404,11 @@ __global__ void __launch_bounds__(128, (MmaCfg<D, MT, BITS4>::CTAS > 2 && MT == 
           top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
         }
         // (m = -inf: any finite maximum is above it)
-        const bool grew = top[0] > m[mt][0] + 8.f || top[1] > m[mt][1] + 8.f;
+        const bool grew = top[0] > m[mt][0] + (kGrow + H::kLift) || top[1] > m[mt][1] + (kGrow + H::kLift);
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float now = fmaxf(m[mt][h], top[h]);
+            const float now = fmaxf(m[mt][h], top[h] - H::kLift);
             const float f = m[mt][h] == kNegInf ? 0.f : exp2_fast(m[mt][h] - now);
             m[mt][h] = now;
             l[mt][h] *= f;

@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(128, Q4Cfg<D>::CTAS) paged_attn_q4_kernel(cons
           for (int e = 0; e < 4; ++e) S[kb][e] *= a.scale_log2;
       }
 
-      // running maximum (a rescaling only when it grew by more than 8)
+      // running maximum (paged_math.cuh)
       float top[2];
       bool grew = false;
 #pragma unroll
@@ -263,12 +263,12 @@ __global__ void __launch_bounds__(128, Q4Cfg<D>::CTAS) paged_attn_q4_kernel(cons
         top[h] = fmaxf(fmaxf(S[0][h], S[0][2 + h]), fmaxf(S[1][h], S[1][2 + h]));
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], o));
-        grew = grew || top[h] > m[h] + 8.f;
+        grew = grew || top[h] > m[h] + (kGrow + H::kLift);
       }
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float now = fmaxf(m[h], top[h]);
+          const float now = fmaxf(m[h], top[h] - H::kLift);
           const float f = m[h] == kNegInf ? 0.f : exp2_fast(m[h] - now);
           m[h] = now;
           l[h] *= f;

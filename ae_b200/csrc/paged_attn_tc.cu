@@ -707,10 +707,9 @@ __global__ void __launch_bounds__(BITS4 ? kTThreads4 : kTThreads, 1)
             for (int e = 0; e < 32; e += 2)
               top[(e >> 1) & 3] = max3(top[(e >> 1) & 3], __uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1]));
           const float tmax = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
-          // a row is rescaled only when its maximum grew by more than 8 (p stays below 2^8)
-          const bool grew = tmax > m + 8.f;
+          const bool grew = tmax > m + (kGrow + H::kLift);  // (paged_math.cuh)
           if (__any_sync(0xffffffffu, grew)) {
-            const float now = grew ? tmax : m;
+            const float now = grew ? tmax - H::kLift : m;
             const float f = m == kNegInf ? 0.f : exp2_fast(m - now);
             m = now;
             l *= f;

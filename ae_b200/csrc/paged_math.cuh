@@ -39,6 +39,12 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// A row's running maximum m is raised when a score passes it by more than kGrow + kLift (base-2 units), and then to
+// that score less kLift: most tiles skip the rescaling, and the weights p = 2^(score - m) stay below
+// 2^(kGrow + kLift).  fp16 ends at 2^16 and loses places below 2^-14, so its weights are lifted by 2^7: they keep their
+// relative precision down to 2^-21 of the row's largest (2^-14 without), and are off by 2^-32 of it at most below.
+constexpr float kGrow = 8.f;
+
 template <typename T>
 struct Half2;
 template <>
@@ -56,6 +62,7 @@ struct Half2<__nv_bfloat16> {
   static constexpr uint32_t kMask = 0x00780078u, kBase = 0x41804180u;
   static constexpr int kUp = 3;
   static constexpr float kMost = 3.38953138925153547590e38f;  // the largest finite number
+  static constexpr float kLift = 0.f;
   static __device__ __forceinline__ uint32_t towards_zero(float x) { return __bfloat16_as_ushort(__float2bfloat16_rz(x)); }
   static __device__ __forceinline__ uint32_t dequant(uint32_t v, uint32_t s2, uint32_t z2) {
     const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&v);
@@ -83,6 +90,7 @@ struct Half2<__half> {
   static constexpr uint32_t kMask = 0x03C003C0u, kBase = 0x4C004C00u;
   static constexpr int kUp = 6;
   static constexpr float kMost = 65504.f;  // the largest finite number
+  static constexpr float kLift = 7.f;
   static __device__ __forceinline__ uint32_t towards_zero(float x) { return __half_as_ushort(__float2half_rz(x)); }
   static __device__ __forceinline__ uint32_t dequant(uint32_t v, uint32_t s2, uint32_t z2) {
     const __half2 x = *reinterpret_cast<const __half2*>(&v);

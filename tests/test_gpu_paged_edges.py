@@ -162,3 +162,41 @@ def test_nonfinite_values_in_every_masked_tile_again_and_again(heads, bits):
         out, lse = call(d)
         assert torch.equal(lse, good_lse) and torch.equal(out[~bad], good[~bad])
         assert not bool(torch.isfinite(out[bad]).any())
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("dtype", [FP, BF], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("heads,D", [(2, 64), (16, 64), (32, 128), (32, 256), (64, 64), (64, 128), (256, 128)])
+def test_many_small_weights_beside_large_ones(heads, D, dtype, bits):
+    """Each 61st key has a weight of 1 and values of 0, the others weights of 2^-26 to 2^-20 and values of 30000, so
+    that the output is theirs alone.
+
+    fp16 has no 2^-26: a weight is kept at 2^7 of its size relative to the row's largest or more, and rounded to a
+    multiple of 2^-24 there where it is below 2^-14: off by 2^-32 at most, of values of 30000, relative to the
+    sum of the weights.  The rest as in ``tests/test_gpu_paged.py``."""
+    N, n = 3000, 2
+    d = make_batch([n], [N], heads, 2, D, 16, dtype, bits, False, seed=13)
+    pages = d["k_cache"].shape[0]
+    g = torch.Generator(device="cuda").manual_seed(14)
+    k = torch.zeros(pages, 2, 16, D, dtype=torch.float64, device="cuda")
+    v = torch.full_like(k, 30000.0)
+    place = torch.zeros(pages * 16, dtype=torch.long, device="cuda")
+    for b, p in enumerate(d["block_table"][0].tolist()):
+        place[p * 16:p * 16 + 16] = torch.arange(b * 16, b * 16 + 16, device="cuda")
+    large = (place.view(pages, 1, 16) % 61 == 0).expand(pages, 2, 16)
+    k[..., 0] = torch.where(large, 0.0, -14 - 4 * torch.rand(pages, 2, 16, generator=g, device="cuda", dtype=torch.float64))
+    v[large] = 0
+    d["k_cache"], d["v_cache"] = ((ref.quantise(t, dtype)[0] if bits == 4 else t.to(dtype)) for t in (k, v))
+    d["q"].zero_()
+    d["q"][..., 0] = 1
+    out, lse = call(d, scale=1.0)
+    o, l, spread, reach = ref.attention(d["q"], d["k_cache"], d["v_cache"], d["block_table"], d["kv_lens"], d["q_starts"],
+                                        scale=1.0)
+    u = ref.half_step(dtype)
+    off = u * reach if bits == 4 and heads > 32 and D <= 128 else torch.zeros_like(reach)
+    lost = N * 2.0 ** -32 * 30000 / torch.exp(l) if dtype == FP else torch.zeros_like(l)  # (the largest score is 0)
+    tol = u * o.abs() + (2 * u + 2 ** -14 + torch.expm1(2 * off)[..., None]) * spread + lost[..., None] + 2 ** -25
+    err = (out.double() - o).abs()
+    assert float(lost.max()) < 0.02 * float(o.abs().min())
+    assert bool((err <= tol).all()), float((err / tol).max())
+    assert bool(((lse.double() - l).abs() <= 2 ** -17 * (l.abs() + 8) + off).all())
