@@ -61,7 +61,7 @@ struct MmaCfg {
   static constexpr int KS = BITS4 ? 32 : 16;       // keys of a warp's stage
   static constexpr int BK = 4 * KS;                // keys of a CTA's tile
   static constexpr int ROW = BITS4 ? kv4_row_bytes(D) : 2 * D;
-  static constexpr int NST = BITS4 ? 4 : (D == 256 ? 3 : 3);
+  static constexpr int NST = BITS4 ? 4 : 3;
   static constexpr int STAGE = 2 * KS * ROW;
   static constexpr int QF = MT * (D / 16) * 512;   // query fragments in fragment order
   static constexpr int RING = 4 * NST * STAGE;
