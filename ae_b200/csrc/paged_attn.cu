@@ -8,8 +8,8 @@
 // memory at these sizes: a key head's rows are read once for all of its g query heads and all
 // new tokens (up to 16 or 32 rows), so the kernel is built to stream.
 //
-// Measured: 32 sequences of up to 32768 keys, one token, 32 / 8 heads of 128, fp16: 2.77 GB in 427-440 us,
-// 6.3-6.5 TB/s, 0.96-0.99 of the measured copy rate.
+// Measured: 32 sequences of up to 32768 keys, one token, 32 / 8 heads of 128, fp16: 2.77 GB in 427-448 us,
+// 6.2-6.5 TB/s, 0.94-0.99 of the measured copy rate.
 //
 // A warp owns a ring of NST stages in shared memory, KS keys each (K and V rows), filled by its
 // own cp.async and read only by itself: no CTA barrier while keys stream, the four warps of a CTA

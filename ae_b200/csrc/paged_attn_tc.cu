@@ -18,11 +18,14 @@
 //    the end.  Bound by memory at the sizes of a verify step: a 64 KB tile takes an SM's share of HBM
 //    about 2800 clocks, twice what its products and exponentials take.
 //
-// Measured (sustained, under the power cap): 16 sequences of up to 16384 keys, trees of 32 tokens, 48 / 8
-// heads of 128: 707 MB of cache and 109 GFLOP in 190-225 us (3.1-3.7 TB/s); two chunks of 2048 tokens
-// over 8191 keys: 290 GFLOP in 295-370 us (785-985 TFLOP/s, with the SM clock).  A 128-key tile of a
-// stream takes about 3250 clocks (clock stamps): 280 to read S, 240 for the maximum, 1420 for the
-// exponentials and P, 1250 until the next S; the two streams' exponentials alone need 2048.
+// Measured, both with two row tiles: 16 sequences of up to 16384 keys, trees of 32 tokens, 48 / 8
+// heads of 128: 707 MB of cache and 109 GFLOP in 187-225 us (3.1-3.8 TB/s); two chunks of 2048 tokens
+// over 8191 keys: 290 GFLOP in 289-370 us (785-1005 TFLOP/s).  Both follow the SM clock (355 and 588 thousand
+// clocks a call; the power cap takes it from 1965 to 1590 and 1785 MHz back to back), so what bounds them is the
+// chain of a tile: about 3400 clocks for a 128-key tile of a stream (clock stamps), 400 to read S, 280 for the
+// maximum, 1400 for the exponentials and P, 1300 until the next S; the two streams' exponentials alone need
+// 2048.  With one row tile: 16 sequences of 8192 keys, trees of 32 tokens, 32 / 8 heads of 128: 537 MB in 105 us,
+// 0.79 of the measured copy rate.
 //
 // Keys and values come by TMA, one box per page (its rows of one head) and 64 dims, into a ring of
 // five 128-row slots with the 128-byte swizzle.  Keys past the end and pages outside the cache are
@@ -35,7 +38,7 @@
 // products with Q are done, so that a segment's first S is there when its predecessor's output has been
 // written.
 //
-// A 4-bit cache (32 / 8 heads, else as above: 73 GFLOP in 205-216 us, bound by the unpacking, 2000 clocks for the
+// A 4-bit cache (32 / 8 heads, else as above: 73 GFLOP in 205-209 us, bound by the unpacking, 2000 clocks for the
 // 128 rows of a slot) has four more warps in the place of TMA's K and V: rows come packed by cp.async into a
 // ring of each warp's own, and go as values of the 16-bit type into the slots (scale x code + zero,
 // one rounding: the score of a key is then off by at most half a step of each of its values, as if the
