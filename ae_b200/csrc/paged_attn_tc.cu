@@ -808,9 +808,8 @@ __global__ void __launch_bounds__(BITS4 ? kTThreads4 : kTThreads, 1)
                   float f;
                   int at = e;
                   if constexpr (BITS4) {
-                    const T* sz = reinterpret_cast<const T*>(v + D / 2 + q * 4);
-                    const int code = (v[q * 16 + e / 2] >> (4 * (e & 1))) & 15;
-                    f = to_f32<T>(from_f32<T>(fmaf(static_cast<float>(code), to_f32<T>(sz[0]), to_f32<T>(sz[1]))));
+                    const uint32_t sz = *reinterpret_cast<const uint32_t*>(v + D / 2 + q * 4);
+                    f = H::lo(value_of<T>((v[q * 16 + e / 2] >> (4 * (e & 1))) & 15u, sz));  // (as it was unpacked)
                     at = (e & ~7) + nibble_place(e & 7);
                   } else {
                     f = to_f32<T>(reinterpret_cast<const T*>(v)[q * 32 + e]);

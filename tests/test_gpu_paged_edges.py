@@ -200,3 +200,23 @@ def test_many_small_weights_beside_large_ones(heads, D, dtype, bits):
     assert float(lost.max()) < 0.02 * float(o.abs().min())
     assert bool((err <= tol).all()), float((err / tol).max())
     assert bool(((lse.double() - l).abs() <= 2 ** -17 * (l.abs() + 8) + off).all())
+
+
+@pytest.mark.parametrize("tree", [False, True], ids=["causal", "tree"])
+@pytest.mark.parametrize("heads", HEADS)
+def test_a_value_just_below_the_overflow_is_finite_in_every_kernel(heads, tree):
+    """15 * 4368 - 2^-24 lies below the middle of 65504 and the next step, so the nearest fp16 is 65504 (rounded to 32
+    bits first it would be the middle, and then infinite), also where another group of the token is not finite."""
+    D = 128
+    d, sees = masked_batch(heads, D, FP, tree)
+    good, _ = call(d)
+    spoil(d, D, FP, 4368.0, -2.0 ** -24)
+    j = 70 - 2
+    row = d["v_cache"][int(d["block_table"][0, j // 16]), :, j % 16]
+    row[:, D // 2 + 12:D // 2 + 16] = torch.tensor([1.0, math.inf], device="cuda").to(FP).view(torch.uint8)
+    out, _ = call(d)
+    for i in range(9):
+        if i not in sees:
+            assert torch.equal(out[i], good[i]), i
+        else:
+            assert bool(torch.isfinite(out[i, :, :96]).all()) and bool(torch.isposinf(out[i, :, 96:]).all()), i
