@@ -155,6 +155,20 @@ def _cache(k: torch.Tensor, v: torch.Tensor, head_dim: int, dtype: torch.dtype, 
     return k.data_ptr(), v.data_ptr(), pages, ps, hs, ts, heads, size, head_dim, bits
 
 
+@functools.lru_cache(maxsize=1024)
+def _cache_rows_overlap(sizes, row: int) -> bool:
+    """Whether rows of ``row`` bytes run into one another; ``sizes``: (pages, page stride, head stride, token stride,
+    heads, page size), strides in bytes."""
+    pages, ps, hs, ts, heads, size = sizes
+    end = row
+    for stride, n in sorted(((ps, pages), (hs, heads), (ts, size))):
+        if n > 1:
+            if stride < end:
+                return True
+            end += stride * (n - 1)
+    return False
+
+
 def _rows(name: str, t: torch.Tensor, shape, dtype: torch.dtype, dev: int):
     """Checks [n, heads, head_dim] rows (the first two strides are free); returns those strides."""
     if t.shape != shape:
@@ -259,7 +273,7 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
 
     q ``[N, Hq, head_dim]``, k and v ``[N, kv_heads, head_dim]`` (views of the projection's output are
     taken as they are).  ``slots`` int64 [N]: where each token goes; negative: nowhere.  The slots of
-    a call have to be distinct.  ``positions`` int64 [N] and ``inv_freq`` float64 [rot / 2]
+    a call, and the rows of the cache, have to be distinct.  ``positions`` int64 [N] and ``inv_freq`` float64 [rot / 2]
     (:func:`rope_inv_freq`) rotate the first ``rot`` dims: pairs (i, i + rot/2), or (2i, 2i + 1) when
     ``interleaved``; both None: no rotation.  ``q_norm`` / ``k_norm`` [head_dim]: weights of an RMS norm
     of each head before the rotation.  Values that fit the type stay finite in a 4-bit cache; a group
@@ -290,8 +304,11 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
         for name, t in (("q", q), ("k", k), ("v", v)):
             if _overlap(out, t):
                 raise ValueError(f"out may not overlap {name}")
-    if N > 0 and cache[2] > 0 and cache[0] == cache[1]:
-        raise ValueError("k_cache and v_cache may not be the same array")
+    if N > 0 and cache[2] > 0:
+        if cache[0] == cache[1]:
+            raise ValueError("k_cache and v_cache may not be the same array")
+        if _cache_rows_overlap(cache[2:8], 2 * D if cache[9] == 16 else kv4_row_bytes(D)):
+            raise ValueError("the rows of a cache to append to may not overlap")
     word, mine = _status_word(status, dev)
     args = _native.APPEND_ARGS
     rc = _launch(dev, _native.load().smb_kv_append, args.pack(

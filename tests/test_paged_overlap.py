@@ -74,3 +74,30 @@ def test_append_refuses_an_out_over_its_inputs_and_one_array_for_both():
     with pytest.raises(ValueError, match="same array"):
         paged.kv_append(q, k, v, kc, kc, slots)
     assert torch.equal(paged.kv_append(q, k, v, kc, vc, slots, out=out), q)
+
+
+def test_rows_of_a_cache_that_run_into_one_another():
+    def f(levels, row):
+        (ps, pages), (hs, heads), (ts, size) = levels
+        return paged._cache_rows_overlap((pages, ps, hs, ts, heads, size), row)
+
+    assert not f(((8192, 4), (4096, 2), (256, 16)), 256)           # heads outside tokens
+    assert not f(((8192, 4), (256, 2), (512, 16)), 256)            # tokens outside heads, a token-major pool
+    assert not f(((65536, 4), (256, 2), (768, 16)), 256)           # a slice of its heads
+    assert not f(((0, 1), (0, 1), (80, 16)), 80) and not f(((5, 1), (7, 1), (3, 1)), 256)
+    for bad in (((8192, 4), (0, 2), (256, 16)), ((0, 4), (4096, 2), (256, 16)), ((8192, 4), (4096, 2), (240, 16)),
+                ((8176, 4), (4096, 2), (256, 16)), ((8192, 4), (256, 2), (256, 16))):
+        assert f(bad, 256), bad
+
+
+@pytest.mark.gpu
+def test_append_refuses_a_cache_of_repeated_rows():
+    x = torch.zeros(4, 8, 64, dtype=torch.float16, device="cuda")
+    kc, vc = (t[:, :1].expand(2, 2, 16, 64) for t in paged.new_cache(2, 1, 16, 64, torch.float16, "cuda"))
+    slots = torch.arange(4, device="cuda")
+    with pytest.raises(ValueError, match="rows of a cache"):
+        paged.kv_append(x[:, :4], x[:, 4:6], x[:, 6:], kc, vc, slots)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    out = paged.paged_attention(x[:1, :4].contiguous(), kc, vc, torch.zeros(1, 1, **i32), torch.ones(1, **i32),
+                                torch.tensor([0, 1], **i32))       # (read, it may be)
+    assert bool((out == 0).all())
