@@ -20,9 +20,10 @@
 // copy rate; issue slots 75 % busy).
 //
 // A 4-bit row keeps, for each 32 values, zero = rn(min), scale = rn((max - min) / 15) in the
-// 16-bit type (rounded down if 15 scale + zero would overflow it: 0 to 65504 in fp16) and codes rint((x - zero) / scale) in [0, 15]; the codes are formed with the
-// rounded scale and zero, so their rounding is not added to the codes' own.  A group with a NaN has
-// both NaN, one with an infinity an infinite scale and codes of 0: either way it reads as NaN.
+// 16-bit type (rounded down if 15 scale + zero would overflow it: 0 to 65504 in fp16) and codes
+// rint((x - zero) / scale) in [0, 15]; the codes are formed with the rounded scale and zero, so their
+// rounding is not added to the codes' own.  A group with a NaN has both NaN, one with an infinity an
+// infinite scale and codes of 0: either way it reads as NaN.
 #include <algorithm>
 #include <type_traits>
 

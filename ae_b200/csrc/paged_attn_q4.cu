@@ -8,10 +8,10 @@
 // an SM) and the scales and exponentials are worked on for the rows that exist.  P^T comes from S^T by
 // transposing 8 x 8 blocks in registers (movmatrix).  Measured: 32 sequences of up to 32768 keys, one
 // token, 32 / 8 heads of 128: 865 MB in 269 us, 3.2 TB/s (330 us with the query rows as the 16; rings of
-// 2 / 3 / 4 stages 276 / 268 / 267 us); the
-// integer pipe, which unpacks the codes, is 56 % busy, the issue slots 57 %.  The rest is as in the kernel for more rows: a
-// warp streams keys of its own through its own ring, scores see no rounding of the keys (scales and
-// zeros are applied to each group's product in 32 bits), values are rounded once to the 16-bit type.
+// 2 / 3 / 4 stages 276 / 268 / 267 us); the integer pipe, which unpacks the codes, is 56 % busy, the issue
+// slots 57 %.  The rest is as in the kernel for more rows: a warp streams keys of its own through its own
+// ring, scores see no rounding of the keys (scales and zeros are applied to each group's product in 32
+// bits), values are rounded once to the 16-bit type.
 #include <algorithm>
 #include <type_traits>
 

@@ -1,5 +1,5 @@
-"""Paged cache and attention at the edges of the number formats (ae_b200/paged.py): non-finite values, and values of a 4-bit
-cache that overflow the 16-bit type.
+"""Paged cache and attention at the edges of the number formats (ae_b200/paged.py): non-finite values,
+values of a 4-bit cache that overflow the 16-bit type, and weights below fp16's normal numbers.
 
 A value of a 4-bit cache enters attention's second product as the 16-bit number nearest scale * code + zero.
 Both numbers of a group can be finite and that one not (fp16: 15 * 4368 = 65520 rounds to infinity).  A row that may
@@ -22,7 +22,8 @@ HEADS = [2, 4, 8, 32, 128]
 # scale and zero of a group as fractions of the largest finite number: code 15 overflows (in fp16 the scale that
 # rounding gives the group 0 to 65504; bf16's rounding keeps that one finite), all but code 0, the negative side,
 # and an infinite scale (code 0 is then NaN)
-GROUPS = {"upper": (4368 / 65504, 0.0), "upper bf16": (0.0675, 0.0), "all": (4368 / 65504, 1.0), "lower": (-4368 / 65504, -0.5), "scale": (math.inf, 0.0)}
+GROUPS = {"upper": (4368 / 65504, 0.0), "upper bf16": (0.0675, 0.0), "all": (4368 / 65504, 1.0),
+          "lower": (-4368 / 65504, -0.5), "scale": (math.inf, 0.0)}
 
 
 def masked_batch(heads, D, dtype, tree):
